@@ -337,6 +337,88 @@ int rt_offload_join(void* cuda_stream);
 int rt_host_register(void* ptr, int64_t bytes);
 int rt_host_unregister(void* ptr);
 
+/*
+ * Microscaled formats: 32 consecutive values of a row share one power-of-two scale.  No
+ * counterpart in the reference's package.  With amax the largest magnitude of a block and e its
+ * exponent, stored as the byte e + 127:
+ *   RT_MXINT8  e smallest with amax <= 127 * 2^(e-6), -120 <= e <= 127;
+ *              code = clamp(rint(x * 2^(6-e)), -127, 127), two's complement; value = code * 2^(e-6)
+ *   RT_MXFP4   e smallest with amax <= 6 * 2^e, -126 <= e <= 126; code = sign, 2 exponent bits, 1
+ *              mantissa bit of y = x * 2^-e on the grid 0, .5, 1, 1.5, 2, 3, 4, 6 (two codes per
+ *              byte, the even column in the low half); value = grid value * 2^e
+ *              nearest: ties to the even mantissa bit; stochastic: floor(|y| / s + r16 / 65536) * s,
+ *              s the grid's step at |y| (0.5 below 2, 1 below 4, else 2)
+ *   a block with an infinity or a NaN: scale byte 255, codes 0; its values read as NaN.
+ * Nothing saturates except at the top of the range: MXINT8 at 127 * 2^121, MXFP4 (e = 126) at
+ * 3 * 2^126, so that what is finite stays finite.  Every value is exactly a
+ * bf16 number, so results are defined bit for bit.  r16 is the draw of "Random bits" above with
+ * stream 3 and i = row * padded cols + column of the QUANTISED matrix (the transposed one if transposed).
+ *
+ * Layout, for R rows x C columns, P = C rounded up to whole blocks, B = P / 32:
+ *   codes   R x P bytes (MXINT8), R x P/2 bytes (MXFP4), row after row; columns from C on hold 0
+ *   scales  MXINT8: R rows of B bytes, each row padded to a multiple of 4.
+ *           MXFP4: tiles of 128 rows x 4 blocks, 512 bytes each, the tiles of a row group one after
+ *           the other; inside a tile the byte of row r, block b is (r % 32) * 16 + (r / 32) * 4 + b.
+ *           Bytes of rows and blocks that do not exist are 0.
+ *   Both start on 16-byte boundaries.  rows, cols < 2^31 - 256 and R * P < 2^34 per call.
+ */
+enum { RT_MXINT8 = 0, RT_MXFP4 = 1 };
+enum { RT_ACT_SILU = 0, RT_ACT_GELU = 1, RT_ACT_GELU_TANH = 2 };
+
+typedef struct rt_mx_draws {
+  uint64_t seed;
+  uint32_t tensor_id;
+  uint32_t step;
+} rt_mx_draws;
+
+/* Bytes of the two arrays; negative: an argument error. */
+int64_t rt_mx_codes_bytes(int format, int64_t rows, int64_t cols);
+int64_t rt_mx_scales_bytes(int format, int64_t rows, int64_t cols);
+
+/* Quantise x (rows x cols, row stride ld elements, columns consecutive).  transpose != 0 (MXFP4 only):
+ * quantise the transposed matrix, cols x rows, in blocks along x's rows.  draws == NULL rounds to
+ * nearest, otherwise stochastically (MXFP4 only). */
+int rt_mx_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld, int format,
+                   int transpose, void* codes, void* scales, const rt_mx_draws* draws,
+                   void* cuda_stream);
+/* The values as bf16, fp32 or fp16 (rounded to nearest; finite values beyond fp16's range become
+ * its largest), rows x cols with row stride ld. */
+int rt_mx_dequantize(int format, const void* codes, const void* scales, int64_t rows, int64_t cols,
+                     void* out, int out_dtype, int64_t ld, void* cuda_stream);
+
+/* Gated activation that keeps its inputs in 8 bits: h = act(gate) * up from the exact inputs, and
+ * gate and up as MXINT8, in one pass.  Backward, from what was kept (g8, u8):
+ *   grad_gate = grad_h * u8 * act'(g8), grad_up = grad_h * act(g8).
+ * silu: g / (1 + exp(-g)); gelu: g * Phi(g); gelu_tanh: its tanh approximation.  fp32 arithmetic. */
+int rt_mx_gated_act(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype,
+                    int64_t rows, int64_t cols, int act, void* h, int64_t ld_h, void* gate_codes,
+                    void* gate_scales, void* up_codes, void* up_scales, void* cuda_stream);
+int rt_mx_gated_act_backward(const void* grad_h, int64_t ld_grad, int dtype, int64_t rows,
+                             int64_t cols, int act, const void* gate_codes, const void* gate_scales,
+                             const void* up_codes, const void* up_scales, void* grad_gate,
+                             int64_t ld_gate, void* grad_up, int64_t ld_up, void* cuda_stream);
+
+/*
+ * Weight gradient from a checkpoint: out[n][k] = sum over tokens t of grad_out[t][n] * value of the
+ * MXINT8 matrix at [t][k] (what the reference's linear.py:401-412 computes from a saved 16-bit
+ * input).  Every product is exact, sums are fp32, one rounding to out's type.  accumulate != 0 adds to
+ * out instead (the sum in fp32, rounded once).  grad_out: tokens x n, row stride ld_grad; out: n x k,
+ * row stride ld_out.  workspace: device memory of at least rt_mx_weight_grad_workspace(...) bytes
+ * for the same arguments (0 for bf16 gradients whose rows start on 16-byte boundaries), 16-byte
+ * aligned, in use until the call's work on the stream is done.
+ */
+int64_t rt_mx_weight_grad_workspace(const void* grad_out, int grad_dtype, int64_t ld_grad,
+                                    int64_t tokens, int64_t n, int64_t k);
+int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, const void* codes,
+                      const void* scales, int64_t tokens, int64_t n, int64_t k, void* out,
+                      int out_dtype, int64_t ld_out, int accumulate, void* workspace,
+                      int64_t workspace_bytes, void* cuda_stream);
+
+/* out[m][n] = sum over k of the MXFP4 values a[m][k] * b[n][k]; fp32 sums, one rounding to out's type. */
+int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const void* b_codes,
+                    const void* b_scales, int64_t m, int64_t n, int64_t k, void* out, int out_dtype,
+                    int64_t ld_out, void* cuda_stream);
+
 /* Counters since load: kernels launched by this library, bytes copied H2D and D2H by the
  * offload pipeline. */
 typedef struct rt_stats {

@@ -66,6 +66,14 @@ class Pull(ctypes.Structure):
                 ("base", c_void_p * (MAX_PEERS + 1))]
 
 
+MXINT8, MXFP4 = 0, 1
+ACT_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+class MxDraws(ctypes.Structure):
+    _fields_ = [("seed", c_uint64), ("tensor_id", c_uint32), ("step", c_uint32)]
+
+
 class Stats(ctypes.Structure):
     _fields_ = [("kernel_launches", c_uint64), ("h2d_bytes", c_uint64), ("d2h_bytes", c_uint64),
                 ("h2d_copies", c_uint64), ("d2h_copies", c_uint64)]
@@ -98,6 +106,20 @@ _SIGNATURES = {
     "rt_offload_join": (c_int, [c_void_p]),
     "rt_host_register": (c_int, [c_void_p, c_int64]),
     "rt_host_unregister": (c_int, [c_void_p]),
+    "rt_mx_codes_bytes": (c_int64, [c_int, c_int64, c_int64]),
+    "rt_mx_scales_bytes": (c_int64, [c_int, c_int64, c_int64]),
+    "rt_mx_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p,
+                               ctypes.POINTER(MxDraws), c_void_p]),
+    "rt_mx_dequantize": (c_int, [c_int, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p]),
+    "rt_mx_gated_act": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int64, c_int64, c_int, c_void_p, c_int64,
+                                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "rt_mx_gated_act_backward": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "rt_mx_weight_grad_workspace": (c_int64, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64]),
+    "rt_mx_weight_grad": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
+                                  c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "rt_mxfp4_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
+                                c_int64, c_void_p]),
     "rt_query_stats": (c_int, [ctypes.POINTER(Stats)]),
 }
 EXPORTS = tuple(_SIGNATURES)

@@ -1,0 +1,102 @@
+"""Layers that keep what their backward pass needs in 8 bits.
+
+    y = linear(x, weight, bias)                     # keeps x as MXINT8, weight by reference
+    h = gated_act(gate, up, "silu")                 # keeps gate and up as MXINT8
+    y = linear(x, weight, product="mxfp4", seed=7, step=t)   # 4-bit products forward and for grad_x
+
+Both take part in autograd like their torch counterparts.  The weight gradient comes straight from
+the 8-bit codes (``microscaling.weight_grad``); for a CPU-resident weight it is added to
+``weight.rt_device_grad`` in HBM, where ``AdamW.step`` takes it (``helpers.accumulate_weight_grad``).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import helpers
+from . import microscaling as mx
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, product, seed, tensor_id, step):
+        w = weight if weight.is_cuda else weight.detach().to(x.device, non_blocking=True)
+        if product == "mxfp4":
+            y = mx.mxfp4_matmul(mx.quantize_mxfp4(x), mx.quantize_mxfp4(w), dtype=x.dtype)
+        else:
+            y = x @ w.t()
+        if bias is not None:
+            y = y + bias.to(x.device)
+        keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] or not weight.is_cuda and weight.requires_grad else None
+        ctx.save_for_backward(*((keep.codes, keep.scales) if keep is not None else (None, None)), weight)
+        ctx.x_shape, ctx.x_dtype, ctx.args = tuple(x.shape), x.dtype, (product, seed, tensor_id, step)
+        ctx.bias_like = None if bias is None else {"dtype": bias.dtype, "device": bias.device}
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        codes, scales, weight = ctx.saved_tensors
+        product, seed, tensor_id, step = ctx.args
+        grad = grad if grad.is_contiguous() else grad.contiguous()
+        gx = gw = gb = None
+        if ctx.needs_input_grad[0]:
+            w = weight if weight.is_cuda else weight.detach().to(grad.device, non_blocking=True)
+            if product == "mxfp4":
+                d4 = mx.quantize_mxfp4(grad, seed=seed, tensor_id=tensor_id, step=step)
+                gx = mx.mxfp4_matmul(d4, mx.quantize_mxfp4(w, transpose=True), dtype=ctx.x_dtype)
+            else:
+                gx = grad @ w
+        if codes is not None:
+            x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
+            if weight.is_cuda:
+                gw = mx.weight_grad(grad, x8, dtype=weight.dtype)
+            else:
+                helpers.accumulate_weight_grad(weight, grad, x8)
+        if ctx.bias_like is not None and ctx.needs_input_grad[2]:
+            gb = grad.reshape(-1, grad.shape[-1]).sum(0, dtype=torch.float32).to(**ctx.bias_like)
+        return gx, gw, gb, None, None, None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, product: str | None = None,
+           seed: int | None = None, tensor_id: int = 0, step: int = 0) -> torch.Tensor:
+    """``x @ weight.T + bias`` that keeps ``x`` in MXINT8 for the weight gradient.
+
+    ``product=None``: the product and ``grad_x`` in x's own type.  ``product="mxfp4"``: both in 4-bit
+    microscaled floating point; the incoming gradient is rounded to 4 bits stochastically when
+    ``seed`` is given (Philox draws ``(seed, tensor_id, step)``: pass another ``tensor_id`` for each layer
+    and count ``step``), else to nearest.  The weight gradient always takes the gradient unrounded.
+
+    A weight in host memory (``is_ramtorch`` parameters) is copied to x's device for the product, and
+    its gradient stays there as ``weight.rt_device_grad``."""
+    if product not in (None, "mxfp4"):
+        raise ValueError(f"product must be None or 'mxfp4', not {product!r}")
+    if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
+    if x.dtype != weight.dtype:
+        raise ValueError(f"x is {x.dtype} and weight {weight.dtype}")
+    if not x.is_cuda:
+        raise RuntimeError("x must be a CUDA tensor: ramtorch_b200 has no CPU implementation")
+    return _Linear.apply(x, weight, bias, product, seed, tensor_id, step)
+
+
+class _GatedAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, up, act):
+        h, g8, u8 = mx.gated_act(gate, up, act)
+        ctx.save_for_backward(g8.codes, g8.scales, u8.codes, u8.scales)
+        ctx.shape, ctx.dtype, ctx.act = tuple(gate.shape), gate.dtype, act
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        gc, gs, uc, us = ctx.saved_tensors
+        g8 = mx.MxTensor("mxint8", gc, gs, ctx.shape, ctx.dtype)
+        u8 = mx.MxTensor("mxint8", uc, us, ctx.shape, ctx.dtype)
+        dgate, dup = mx.gated_act_backward(grad if grad.is_contiguous() else grad.contiguous(), g8, u8, ctx.act)
+        return dgate, dup, None
+
+
+def gated_act(gate: torch.Tensor, up: torch.Tensor, act: str = "silu") -> torch.Tensor:
+    """``act(gate) * up`` that keeps its two inputs in MXINT8 (``act``: ``"silu"``, ``"gelu"``, ``"gelu_tanh"``)."""
+    return _GatedAct.apply(gate, up, act)

@@ -12,13 +12,15 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 ROOT = os.path.dirname(PKG)
 OUT = os.path.join(PKG, "librt_b200.so")
-SOURCES = ["adamw_sr.cu", "offload.cu"]
-DEPS = SOURCES + ["philox.cuh", "rt_internal.h", os.path.join(ROOT, "include", "rt_b200.h")]
+OBJ = os.path.join(HERE, "_obj")
+SOURCES = ["adamw_sr.cu", "offload.cu", "microscale.cu", "mx_gemm.cu"]
+DEPS = SOURCES + ["philox.cuh", "mx_common.cuh", "rt_internal.h", os.path.join(ROOT, "include", "rt_b200.h")]
 
 
 def nvcc_path() -> str:
@@ -43,16 +45,29 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return OUT
     nvcc = nvcc_path()
     cuda_lib = os.path.join(os.path.dirname(os.path.dirname(nvcc)), "lib64")
-    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-Xcompiler", "-fPIC,-O2,-Wall", "-shared", "-cudart", "shared",
-           "-Xlinker", f"-rpath={cuda_lib}", "-o", OUT + ".tmp"]
+    arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
+    flags = arch + ["-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-O2,-Wall"]
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += [os.path.join(HERE, s) for s in SOURCES]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-    if res.returncode != 0:
+        flags += ["-Xptxas", "-v"]
+    os.makedirs(OBJ, exist_ok=True)
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+        return res.returncode
+
+    def compile_one(name):      # one translation unit at a time per thread; unchanged ones keep their object
+        src, obj = os.path.join(HERE, name), os.path.join(OBJ, name[:-3] + ".o")
+        newest = max(os.path.getmtime(os.path.join(HERE, d)) for d in [name] + [d for d in DEPS if not d.endswith(".cu")])
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) > newest:
+            return 0, obj
+        return run([nvcc, *flags, "-c", src, "-o", obj]), obj
+
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        done = list(pool.map(compile_one, SOURCES))
+    link = [nvcc, *arch, "-shared", "-cudart", "shared", "-Xlinker", f"-rpath={cuda_lib}", "-o", OUT + ".tmp"]
+    if any(rc for rc, _ in done) or run(link + [obj for _, obj in done]):
         raise RuntimeError("nvcc failed building librt_b200.so")
     os.replace(OUT + ".tmp", OUT)
     return OUT

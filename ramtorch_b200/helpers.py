@@ -99,3 +99,21 @@ def accumulate_device_grad(param: torch.Tensor, grad: torch.Tensor) -> torch.Ten
     else:
         held.add_(grad.detach())
     return held
+
+
+def accumulate_weight_grad(param: torch.Tensor, grad_out: torch.Tensor, x8) -> torch.Tensor:
+    """:func:`accumulate_device_grad` of a linear layer's weight gradient that is formed on the way:
+    ``grad_out.T @ x8`` from the layer's input as an MXINT8 checkpoint (``microscaling.quantize_mxint8``).
+    The first micro-batch stores it in the parameter's dtype, later ones add in fp32 before the
+    one rounding.  With ZeRO-2 hooks on the parameter the fresh gradient passes through them first
+    (linear.py:409-414), then is added.  Returns the accumulated gradient."""
+    from . import microscaling as mx
+    if not grad_out.is_cuda:
+        raise ValueError("accumulate_weight_grad is for gradients that live in HBM")
+    if param.dim() != 2 or tuple(param.shape) != (grad_out.shape[-1], x8.shape[-1]):
+        raise ValueError("gradient and parameter shapes differ")
+    held = param.__dict__.get(DEVICE_GRAD_ATTR)
+    if held is not None and not getattr(param, ZERO2_HOOK_NAME, None):
+        return mx.weight_grad(grad_out, x8, out=held, accumulate=True)
+    fresh = mx.weight_grad(grad_out, x8, dtype=param.dtype)
+    return accumulate_device_grad(param, invoke_ramtorch_hooks(param, fresh))
