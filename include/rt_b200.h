@@ -414,6 +414,11 @@ int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, con
                       int out_dtype, int64_t ld_out, int accumulate, void* workspace,
                       int64_t workspace_bytes, void* cuda_stream);
 
+/* Waits inside the tensor-core kernels that ran out on the current device since load (each is bounded by
+ * two seconds so that a fault ends the kernel instead of hanging the GPU).  0, or the results of a
+ * call are wrong.  Synchronous. */
+int rt_mx_wait_faults(uint32_t* count);
+
 /* out[m][n] = sum over k of the MXFP4 values a[m][k] * b[n][k]; fp32 sums, one rounding to out's type. */
 int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const void* b_codes,
                     const void* b_scales, int64_t m, int64_t n, int64_t k, void* out, int out_dtype,

@@ -118,6 +118,7 @@ _SIGNATURES = {
     "rt_mx_weight_grad_workspace": (c_int64, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64]),
     "rt_mx_weight_grad": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
                                   c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "rt_mx_wait_faults": (c_int, [ctypes.POINTER(c_uint32)]),
     "rt_mxfp4_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
                                 c_int64, c_void_p]),
     "rt_query_stats": (c_int, [ctypes.POINTER(Stats)]),

@@ -20,7 +20,7 @@ ROOT = os.path.dirname(PKG)
 OUT = os.path.join(PKG, "librt_b200.so")
 OBJ = os.path.join(HERE, "_obj")
 SOURCES = ["adamw_sr.cu", "offload.cu", "microscale.cu", "mx_gemm.cu"]
-DEPS = SOURCES + ["philox.cuh", "mx_common.cuh", "rt_internal.h", os.path.join(ROOT, "include", "rt_b200.h")]
+DEPS = SOURCES + ["philox.cuh", "mx_common.cuh", "tc05.cuh", "rt_internal.h", os.path.join(ROOT, "include", "rt_b200.h")]
 
 
 def nvcc_path() -> str:

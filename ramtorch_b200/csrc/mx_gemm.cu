@@ -1,36 +1,304 @@
-// Products of microscaled operands: the weight gradient from an 8-bit checkpoint, and the product
-// of two MXFP4 matrices.
+// Products of microscaled operands on the fifth-generation tensor cores: the weight gradient from
+// an 8-bit checkpoint, and the product of two MXFP4 matrices.
 //
-// Simple form: 64 x 64 outputs per CTA, 16 steps of the sum at a time through shared memory, fp32
-// multiply-adds in registers.  Every value of either format is exactly an fp32 number, so all that is
-// rounded is the sum.
+// Both compute the transposed output tile: the 128 lanes of the accumulator are 128 consecutive
+// columns of the output (weight columns, output features), its columns are output rows.  A warp that reads a
+// column of the accumulator therefore holds 32 neighbours of one output row and stores them in
+// one access, with no transposition on the way out, and the side that varies (tokens of a small batch, rows
+// of a weight) takes the accumulator's columns, where tiles of any multiple of 32 are cheap.
 #include <algorithm>
+#include <atomic>
+
+#include <cudaTypedefs.h>
 
 #include "mx_common.cuh"
+#include "tc05.cuh"
 
 namespace rt {
 
 int mx_check_shape(int64_t rows, int64_t cols);
 int mx_check_codes(const void* codes, const void* scales);
 
-struct FromGradient {       // element (t, i) of a tokens x n gradient
-  const void* p;
-  int dtype;
+__device__ unsigned int g_wait_faults;   // waits that ran out; see rt_mx_wait_faults
+
+constexpr int kSms = 148;
+constexpr int kTcThreads = 384;          // warp 0: loads, 1: products, 2: tensor memory, 4-11: conversion and output
+constexpr int kFirstWorker = 4;
+
+struct OutMatrix {
+  void* p;
   int64_t ld;
-  __device__ float operator()(int64_t t, int64_t i) const {
-    if (dtype == RT_F32) return static_cast<const float*>(p)[t * ld + i];
-    const uint16_t v = static_cast<const uint16_t*>(p)[t * ld + i];
-    return dtype == RT_BF16 ? to_f32<RT_BF16>(v) : to_f32<RT_F16>(v);
-  }
+  int rows, cols;                        // the accumulator's columns / lanes
+  int dtype, accumulate;
 };
-struct FromInt8 {           // element (t, i) of a tokens x k checkpoint
-  const uint8_t* codes;
+
+template <int D>
+__device__ __forceinline__ void put_one(const OutMatrix& o, int64_t at, float v) {
+  elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + at;
+  *p = of_f32<D>(o.accumulate ? to_f32<D>(*p) + v : v);
+}
+__device__ __forceinline__ void put_out(const OutMatrix& o, int64_t at, float v) {
+  if (o.dtype == RT_BF16) put_one<RT_BF16>(o, at, v);
+  else if (o.dtype == RT_F32) put_one<RT_F32>(o, at, v);
+  else put_one<RT_F16>(o, at, v);
+}
+// 32 columns of the accumulator that this warp holds, to 32 output rows
+template <int D>
+__device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col, const uint32_t (&acc)[32]) {
+  if (col >= o.cols) return;
+  elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + (int64_t)row * o.ld + col;
+  const int live = min(32, o.rows - row);
+  if (o.accumulate) {
+    float old[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) old[j] = j < live ? to_f32<D>(p[j * o.ld]) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < live) p[j * o.ld] = of_f32<D>(old[j] + __uint_as_float(acc[j]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < live) p[j * o.ld] = of_f32<D>(__uint_as_float(acc[j]));
+  }
+}
+
+// The worker warps' part after the last product.  One CTA per tile: straight from tensor memory.
+// A cluster per tile (the sum is split over its CTAs): every CTA leaves its part in shared memory, then adds
+// up a share of the tile's columns over all of them, always in the order of their ranks.
+template <int BN>
+__device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, int row0, int col0, int splits, float* parts, bool ok) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
+  const bool worker = warp >= kFirstWorker;
+  if (worker) {
+    constexpr int kHalf = BN >= 64 ? BN / 2 : BN;
+    const int c0 = (warp - kFirstWorker) >= 4 ? kHalf : 0;
+    if (c0 < BN && ok) {
+#pragma unroll 1
+      for (int c = c0; c < c0 + kHalf; c += 32) {
+        uint32_t acc[32];
+        tmem_load32(tmem + ((uint32_t)(q * 32) << 16) + c, acc);
+        if (splits == 1) {
+          if (row0 + c < o.rows) {
+            if (o.dtype == RT_BF16) put_columns<RT_BF16>(o, row0 + c, col0 + q * 32 + lane, acc);
+            else if (o.dtype == RT_F32) put_columns<RT_F32>(o, row0 + c, col0 + q * 32 + lane, acc);
+            else put_columns<RT_F16>(o, row0 + c, col0 + q * 32 + lane, acc);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) parts[(c + j) * 128 + q * 32 + lane] = __uint_as_float(acc[j]);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  if (splits > 1) {
+    __syncwarp();
+    cluster_sync();
+    if (worker) {
+      const int rank = (int)cluster_rank(), i = threadIdx.x - kFirstWorker * 32;
+      const int per = BN / splits;                                    // splits divides 8, BN is a multiple of 32
+      const uint32_t base = smem_u32(parts);
+      const int col = col0 + (i & 127);
+      for (int c = rank * per + (i >> 7); c < (rank + 1) * per; c += 2) {
+        if (row0 + c >= o.rows || col >= o.cols) continue;
+        float v = 0.f;
+        for (int r = 0; r < splits; ++r) v += load_peer(base + (uint32_t)(c * 128 + (i & 127)) * 4, r);
+        put_out(o, (int64_t)(row0 + c) * o.ld + col, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+  }
+}
+
+// ------------------------------------------------------------------------------- weight gradient
+// D[k, n] = sum over tokens of value(k, t) * grad(t, n).  Both operands lie with the token as the
+// slow index, so both are MN-major; a step takes 64 tokens.  The gradient's tile comes by TMA
+// ready for the tensor core; the codes' tile (8 KB) comes by TMA as bytes, the worker warps turn
+// it into bf16 (exact: a code times a power of two) in the swizzled layout.  fp32 and fp16
+// gradients arrive as up to three bf16 pieces that add up to them exactly; the pieces are further steps of the same sum.
+constexpr int kTok = 64;
+
+template <int BN>
+struct WgradSmem {
+  static constexpr int kCodes = 128 * kTok, kA = 128 * kTok * 2, kB = BN * kTok * 2;
+  static constexpr int kStage = kCodes + kA + kB;
+  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 5 : 6;
+  static constexpr int kBytes = kStages * kStage + 1024 + 256;   // alignment, barriers
+};
+
+struct WgradArgs {
   const uint8_t* scales;
-  int64_t ld, ld_scales;
-  __device__ float operator()(int64_t t, int64_t i) const {
-    return (float)(int8_t)codes[t * ld + i] * scale_of(scales[t * ld_scales + (i >> 5)], 6);
-  }
+  int64_t ld_scales;
+  int tokens, blocks;                     // blocks of 32 along k
+  int token_steps, pieces, splits;
+  int k_tiles, n_tiles;
+  OutMatrix out;
 };
+
+// two codes in the low bytes of the halves of a word -> two bf16 integers: with the byte c = low7 - (sign bit),
+// 128 + low7 and 128 + (sign bit) are bf16 numbers made by setting bits, their difference is exact
+__device__ __forceinline__ uint32_t bf16x2_of_codes(uint32_t w, __nv_bfloat162 scale) {
+  const uint32_t x = (w & 0x007F007Fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
+  const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y)), scale);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ __nv_bfloat162 bf16x2_scale(uint32_t byte) {
+  const uint32_t h = byte == 255u ? 0x7FC0u : byte >= 7u ? (byte - 6u) << 7 : 1u << byte;   // 2^(byte - 133)
+  const uint32_t w = h | h << 16;
+  return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kTcThreads, 1)
+mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_grad, const WgradArgs a) {
+  using S = WgradSmem<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t tile_a = base, tile_b = tile_a + S::kStages * S::kA, codes = tile_b + S::kStages * S::kB;
+  const uint32_t bars = codes + S::kStages * S::kCodes;
+  const uint32_t full = bars, empty = bars + 8 * S::kStages, conv = empty + 8 * S::kStages, done = conv + 8 * S::kStages, slot = done + 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // tiles: groups of eight along n, k inside: the CTAs that run together share few tiles of either side
+  const int tile = blockIdx.x / a.splits, rank = blockIdx.x % a.splits;
+  const int per_group = 8 * a.k_tiles, group = tile / per_group, width = min(8, a.n_tiles - 8 * group);
+  const int in_group = tile - group * per_group;
+  const int n0 = (group * 8 + in_group % width) * BN, k0 = (in_group / width) * 128;
+  const int64_t steps = (int64_t)a.token_steps * a.pieces;
+  const int first = (int)(steps * rank / a.splits), last = (int)(steps * (rank + 1) / a.splits);
+
+  if (warp == 0 && elect_one()) {
+    prefetch_map(&map_codes);
+    prefetch_map(&map_grad);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+      mbar_init(conv + 8 * s, 8);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+  }
+  constexpr int kColumns = BN;
+  if (warp == 2) tmem_alloc(slot, kColumns);
+  __syncthreads();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int piece = first / a.token_steps, t = first % a.token_steps, i = 0;
+      for (int it = first; it < last && ok; ++it, ++i) {
+        const int s = i % S::kStages;
+        if (!(ok = mbar_wait(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
+        mbar_expect(full + 8 * s, S::kCodes + S::kB);
+        tma_load_2d(&map_codes, codes + s * S::kCodes, full + 8 * s, k0, t * kTok);
+#pragma unroll
+        for (int j = 0; j < BN / 64; ++j)
+          tma_load_3d(&map_grad, tile_b + s * S::kB + j * 8192, full + 8 * s, n0 + j * 64, t * kTok, piece);
+        if (++t == a.token_steps) { t = 0; ++piece; }
+      }
+      if (!ok)   // the loads in flight still write to this CTA's memory
+        for (int j = 0; j < S::kStages && j < i; ++j) {
+          const int latest = i - 1 - (i - 1 - j) % S::kStages;       // the last step that used stage j
+          mbar_wait(full + 8 * j, (latest / S::kStages) & 1);
+        }
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = idesc_bf16_mn(128, BN);
+      for (int i = 0; i < last - first; ++i) {
+        const int s = i % S::kStages, phase = (i / S::kStages) & 1;
+        if (!(ok = mbar_wait(full + 8 * s, phase) && mbar_wait(conv + 8 * s, phase))) break;
+        tc_fence_after();
+        const uint64_t da = tile_desc(tile_a + s * S::kA, 8192, 1024), db = tile_desc(tile_b + s * S::kB, 8192, 1024);
+#pragma unroll
+        for (int kk = 0; kk < kTok / 16; ++kk) mma_bf16(tmem, da + kk * (2048 >> 4), db + kk * (2048 >> 4), idesc, i > 0 || kk > 0);
+        tc_commit(empty + 8 * s);
+      }
+      tc_commit(done);
+    }
+  } else if (warp >= kFirstWorker) {
+    const int w = threadIdx.x - kFirstWorker * 32;
+    const int tok[2] = {w >> 3, (w + 256) >> 3}, f16 = w & 7;      // 16 codes each: token, sixteenth of the features
+    const int block = (k0 >> 5) + (f16 >> 1);
+    const uint8_t* sc = a.scales + block;
+    const bool has_block = block < a.blocks;
+    const uint32_t dst = (uint32_t)(f16 >> 2) * 8192, flip = (uint32_t)(f16 >> 2);   // the halves of a warp's lanes start with different chunks: no bank conflicts
+    int t = first % a.token_steps;
+    uint32_t byte[2];
+    auto fetch = [&](int step) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int token = step * kTok + tok[h];
+        byte[h] = has_block && token < a.tokens ? __ldg(sc + token * a.ld_scales) : 127u;
+      }
+    };
+    if (first < last) fetch(t);
+    for (int i = 0; i < last - first; ++i) {
+      const int s = i % S::kStages, phase = (i / S::kStages) & 1;
+      const __nv_bfloat162 scale[2] = {bf16x2_scale(byte[0]), bf16x2_scale(byte[1])};
+      if (++t == a.token_steps) t = 0;
+      if (i + 1 < last - first) fetch(t);
+      if (!(ok = mbar_wait(full + 8 * s, phase))) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 c = *reinterpret_cast<const uint4*>(smem + (codes - base) + s * S::kCodes + tok[h] * 128 + f16 * 16);
+        const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+        uint32_t v[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[2 * j] = bf16x2_of_codes(__byte_perm(in[j], 0u, 0x4140), scale[h]);
+          v[2 * j + 1] = bf16x2_of_codes(__byte_perm(in[j], 0u, 0x4342), scale[h]);
+        }
+        uint8_t* row = smem + (tile_a - base) + s * S::kA + dst + tok[h] * 128;
+        const uint32_t c0 = (uint32_t)(f16 & 3) * 2, x = (uint32_t)tok[h] & 7u;
+        const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ x) << 4)) = flip ? hi : lo;
+        *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ x) << 4)) = flip ? lo : hi;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(conv + 8 * s);
+    }
+    ok = mbar_wait(done, 0) && ok;
+    tc_fence_after();
+  }
+  __syncwarp();
+  if (!ok) atomicAdd(&g_wait_faults, 1u);
+  finish_tile<BN>(a.out, tmem, n0, k0, a.splits, reinterpret_cast<float*>(smem), ok);
+  __syncthreads();
+  if (warp == 2) tmem_free(tmem, kColumns);
+}
+
+// A gradient that the tensor maps cannot take as it is (fp32, fp16, rows that do not start on 16-byte
+// boundaries) as bf16 planes whose sum it is: the leading 8 bits of each value's mantissa, the next 8,
+// the rest.  Cut, not rounded, so that nothing overflows; an infinity or a NaN is in the first plane alone.
+template <int D, int P>
+__global__ void __launch_bounds__(256)
+spread_gradient_kernel(const elem_t<D>* __restrict__ g, const int64_t ld, const int64_t tokens, const int n, const int np, uint16_t* __restrict__ planes) {
+  const int64_t total = tokens * np;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / np;
+    const int c = (int)(i - t * np);
+    float v = c < n ? to_f32<D>(g[t * ld + c]) : 0.f;
+    if constexpr (P == 1) {
+      planes[i] = of_f32<RT_BF16>(v);
+    } else {
+      uint32_t b = __float_as_uint(v);
+      const bool odd = (b & 0x7F800000u) == 0x7F800000u;
+      if (odd && (b & 0x7FFFFFu)) b = 0x7FC00000u;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        planes[p * total + i] = (uint16_t)(b >> 16);
+        v = odd ? 0.f : v - __uint_as_float(b & 0xFFFF0000u);
+        b = __float_as_uint(v);
+      }
+    }
+  }
+}
+
 struct FromFp4 {            // element (t, i): column t of row i
   const uint8_t* codes;
   const uint8_t* scales;
@@ -96,6 +364,66 @@ static int launched() {
   return 0;
 }
 
+
+static PFN_cuTensorMapEncodeTiled_v12000 map_encoder() {
+  static std::atomic<void*> fn{nullptr};
+  void* p = fn.load(std::memory_order_acquire);
+  if (!p) {
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+      return nullptr;
+    fn.store(p, std::memory_order_release);
+  }
+  return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+}
+// dims and box from the innermost dimension; strides (bytes) of all but the innermost
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, int rank, const uint64_t* dims, const uint64_t* strides,
+                    const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  auto encode = map_encoder();
+  if (!encode) { cudaGetLastError(); return fail(RT_E_DEVICE, "the driver has no cuTensorMapEncodeTiled"); }
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = encode(map, type, (cuuint32_t)rank, const_cast<void*>(p), reinterpret_cast<const cuuint64_t*>(dims),
+                            reinterpret_cast<const cuuint64_t*>(strides), box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(RT_E_CONFIG, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return 0;
+}
+
+// Launch a tensor-core kernel as clusters of `splits` CTAs.  Its shared memory is raised once per
+// device and kernel.
+template <typename K, typename... Args>
+static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t ctas, int splits, cudaStream_t st, Args... args) {
+  int device = 0;
+  RT_CUDA(cudaGetDevice(&device));
+  if (device >= 64 || !(raised.load(std::memory_order_acquire) >> device & 1)) {
+    RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (device < 64) raised.fetch_or(1ull << device, std::memory_order_release);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)splits;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  RT_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+  stats().kernel_launches.fetch_add(1, std::memory_order_relaxed);
+  return 0;
+}
+
+template <int BN>
+static int run_wgrad(const CUtensorMap& codes, const CUtensorMap& grad, const WgradArgs& a, cudaStream_t st) {
+  static std::atomic<uint64_t> raised{0};
+  return launch_tc(mx_weight_grad_kernel<BN>, raised, WgradSmem<BN>::kBytes, (int64_t)a.k_tiles * a.n_tiles * a.splits, a.splits, st, codes, grad, a);
+}
+
+static int pieces_of(int dtype) { return dtype == RT_F32 ? 3 : dtype == RT_F16 ? 2 : 1; }
+static bool taken_as_is(const void* p, int dtype, int64_t ld) { return dtype == RT_BF16 && aligned16(p, ld, 2); }
+
 }  // namespace rt
 
 using namespace rt;
@@ -104,7 +432,8 @@ extern "C" int64_t rt_mx_weight_grad_workspace(const void* grad_out, int grad_dt
   if (!dtype_ok(grad_dtype)) return fail(RT_E_DTYPE, "dtype code must be 0 (bf16), 1 (f32) or 2 (f16)");
   if (int rc = mx_check_shape(tokens, k)) return rc;
   if (int rc = mx_check_shape(tokens, n)) return rc;
-  return 0;
+  if (tokens == 0 || n == 0 || k == 0 || taken_as_is(grad_out, grad_dtype, ld_grad)) return 0;
+  return pieces_of(grad_dtype) * tokens * pad_to(n, 8) * 2;
 }
 
 extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, const void* codes, const void* scales,
@@ -115,19 +444,82 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   if (n == 0 || k == 0) return 0;
   if (int rc = check_out(out, out_dtype, k, ld_out)) return rc;
   if (!dtype_ok(grad_dtype)) return fail(RT_E_DTYPE, "dtype code must be 0 (bf16), 1 (f32) or 2 (f16)");
-  if (tokens > 0) {
-    if (!grad_out) return fail(RT_E_NULL, "grad_out must be non-null");
-    if (ld_grad < n || ld_grad > ((int64_t)1 << 40)) return fail(RT_E_SIZE, "row stride of grad_out must be >= n and at most 2^40");
-    if ((uintptr_t)grad_out % dtype_size(grad_dtype)) return fail(RT_E_ALIGN, "grad_out is not aligned to its element size");
-    if (int rc = mx_check_codes(codes, scales)) return rc;
+  cudaStream_t st = (cudaStream_t)cuda_stream;
+  if (tokens == 0) {                        // an empty sum
+    const size_t size = dtype_size(out_dtype);
+    if (!accumulate) RT_CUDA(cudaMemset2DAsync(out, ld_out * size, 0, k * size, n, st));
+    return 0;
   }
-  const int64_t kp = pad_to(k, kMxBlock);
-  const FromGradient a{grad_out, grad_dtype, ld_grad};
-  const FromInt8 b{(const uint8_t*)codes, (const uint8_t*)scales, kp, pad_to(kp / kMxBlock, 4)};
-  const dim3 grid((unsigned)((k + 63) / 64), (unsigned)((n + 63) / 64));
-  if (grid.y > 65535) return fail(RT_E_SIZE, "n too large");
-  simple_product_kernel<<<grid, 256, 0, (cudaStream_t)cuda_stream>>>(a, b, tokens, n, k, out, out_dtype, ld_out, accumulate);
-  return launched();
+  if (!grad_out) return fail(RT_E_NULL, "grad_out must be non-null");
+  if (ld_grad < n || ld_grad > ((int64_t)1 << 38)) return fail(RT_E_SIZE, "row stride of grad_out must be >= n and at most 2^38");
+  if ((uintptr_t)grad_out % dtype_size(grad_dtype)) return fail(RT_E_ALIGN, "grad_out is not aligned to its element size");
+  if (int rc = mx_check_codes(codes, scales)) return rc;
+  const int64_t need = rt_mx_weight_grad_workspace(grad_out, grad_dtype, ld_grad, tokens, n, k);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need) return fail(RT_E_CONFIG, "workspace is smaller than rt_mx_weight_grad_workspace says");
+    if ((uintptr_t)workspace & 15) return fail(RT_E_ALIGN, "workspace must be 16-byte aligned");
+  }
+
+  const int64_t np = pad_to(n, 8), kp = pad_to(k, kMxBlock);
+  const int pieces = need ? pieces_of(grad_dtype) : 1;
+  WgradArgs a{};
+  a.scales = (const uint8_t*)scales;
+  a.blocks = (int)(kp / kMxBlock);
+  a.ld_scales = pad_to(a.blocks, 4);
+  a.tokens = (int)tokens;
+  a.token_steps = (int)((tokens + kTok - 1) / kTok);
+  a.pieces = pieces;
+  a.out = {out, ld_out, (int)n, (int)k, out_dtype, accumulate != 0};
+
+  // Tile width and split.  A step costs what the longer of the product and the conversion costs;
+  // a CTA also pays for its start, its output and, when split, the exchange (clocks, measured).
+  const int64_t steps = (int64_t)a.token_steps * pieces;
+  const int64_t k_tiles = (k + 127) / 128;
+  int bn = 256, splits = 1;
+  double best = 1e300;
+  for (const int width : {256, 128, 64})
+    for (const int s : {1, 2, 4, 8}) {
+      if (s > steps) continue;
+      const double step = width == 256 ? 700 : width == 128 ? 400 : 300;
+      const int64_t ctas = k_tiles * ((n + width - 1) / width) * s;
+      const double cost = (double)((ctas + kSms - 1) / kSms) * ((double)((steps + s - 1) / s) * step + 3000 + width * 12 + (s > 1 ? 2500 : 0));
+      if (cost < best) { best = cost; bn = width; splits = s; }
+    }
+  a.splits = splits;
+  a.k_tiles = (int)k_tiles;
+  a.n_tiles = (int)((n + bn - 1) / bn);
+  if (k_tiles * a.n_tiles * splits > 0x7FFFFFFFll) return fail(RT_E_SIZE, "n * k is too large");
+
+  CUtensorMap map_codes, map_grad;
+  {
+    const uint64_t dims[2] = {(uint64_t)kp, (uint64_t)tokens}, strides[1] = {(uint64_t)kp};
+    const uint32_t box[2] = {128, (uint32_t)kTok};
+    if (int rc = make_map(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+  }
+  {
+    const int64_t ld = need ? np : ld_grad;
+    const uint64_t dims[3] = {(uint64_t)n, (uint64_t)tokens, (uint64_t)pieces}, strides[2] = {(uint64_t)ld * 2, (uint64_t)(need ? tokens * np * 2 : ld * 2)};
+    const uint32_t box[3] = {64, (uint32_t)kTok, 1};
+    if (int rc = make_map(&map_grad, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, need ? workspace : grad_out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  if (need) {
+    const unsigned nb = (unsigned)std::min<int64_t>((tokens * np + 255) / 256, kSms * 16);
+    if (grad_dtype == RT_F32) spread_gradient_kernel<RT_F32, 3><<<nb, 256, 0, st>>>((const float*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
+    else if (grad_dtype == RT_F16) spread_gradient_kernel<RT_F16, 2><<<nb, 256, 0, st>>>((const uint16_t*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
+    else spread_gradient_kernel<RT_BF16, 1><<<nb, 256, 0, st>>>((const uint16_t*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
+    if (int rc = launched()) return rc;
+  }
+  if (bn == 256) return run_wgrad<256>(map_codes, map_grad, a, st);
+  if (bn == 128) return run_wgrad<128>(map_codes, map_grad, a, st);
+  return run_wgrad<64>(map_codes, map_grad, a, st);
+}
+
+extern "C" int rt_mx_wait_faults(uint32_t* count) {
+  if (!count) return fail(RT_E_NULL, "count must be non-null");
+  unsigned int v = 0;
+  RT_CUDA(cudaMemcpyFromSymbol(&v, g_wait_faults, sizeof v));
+  *count = v;
+  return 0;
 }
 
 extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales, int64_t m,

@@ -593,3 +593,10 @@ def test_repeated_calls_give_the_same_bits():
     first = mx.weight_grad(g, q), mx.mxfp4_matmul(a, b)
     for _ in range(3):
         assert torch.equal(first[0], mx.weight_grad(g, q)) and torch.equal(first[1], mx.mxfp4_matmul(a, b))
+
+
+@gpu
+def test_no_wait_ran_out():
+    torch.cuda.synchronize()
+    count = ctypes.c_uint32(99)
+    assert N.lib().rt_mx_wait_faults(ctypes.byref(count)) == 0 and count.value == 0
