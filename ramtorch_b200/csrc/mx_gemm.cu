@@ -299,56 +299,116 @@ spread_gradient_kernel(const elem_t<D>* __restrict__ g, const int64_t ld, const 
   }
 }
 
-struct FromFp4 {            // element (t, i): column t of row i
-  const uint8_t* codes;
-  const uint8_t* scales;
-  int64_t ld;
-  int ktiles;
-  __device__ float operator()(int64_t t, int64_t i) const {
-    const uint32_t c = codes[i * ld + (t >> 1)] >> (4 * (t & 1));
-    const float v = __uint_as_float((c & 7u) << 22) * 0x1p126f * scale_of(scales[fp4_scale_at(i, (int)(t >> 5), ktiles)], 0);
-    return c & 8u ? -v : v;
-  }
+// ---------------------------------------------------------------------------------- fp4 product
+// D[n, m] = sum over k of b[n, k] * a[m, k]: the 128 lanes are rows of b (output features), the
+// columns rows of a (tokens).  Codes go from global memory to the tensor core as they are stored: a
+// step is 256 columns, 128 bytes of a row, K-major.  The scales lie in global memory in the order
+// that tensor memory wants, so a row tile's scales of a step are one bulk copy to shared memory and
+// two copies (one per 128 columns) to tensor memory, where each stage has columns of its own.
+// The product takes a tile's scales from where a scale tile begins (an odd column of tensor memory
+// is a misaligned address to it), so narrow tiles serve only matrices of a single tile of rows.
+constexpr int kStepK = 256;
+
+template <int BN>
+struct Fp4Smem {
+  static constexpr int kA = 128 * 128, kB = BN * 128, kScale = 1024;
+  static constexpr int kStage = kA + kB + 2 * kScale;
+  static constexpr int kStages = BN == 128 ? 3 : BN == 64 ? 4 : 5;   // two CTAs to an SM
+  static constexpr int kBytes = kStages * kStage + 1024 + 256;
+  static constexpr int kColumns = BN + 16 * kStages <= 128 ? 128 : 256;
 };
 
-template <typename A, typename B>
-__global__ void __launch_bounds__(256)
-simple_product_kernel(const A a, const B b, const int64_t depth, const int64_t rows, const int64_t cols, void* out, const int out_dtype,
-                      const int64_t ld, const int accumulate) {
-  __shared__ float sa[16][65], sb[16][65];
-  const int64_t i0 = (int64_t)blockIdx.y * 64, j0 = (int64_t)blockIdx.x * 64;
-  const int ti = threadIdx.x >> 4, tj = threadIdx.x & 15;
-  float acc[4][4] = {};
-  for (int64_t t0 = 0; t0 < depth; t0 += 16) {
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-      const int t = e >> 6, i = e & 63;
-      const bool live = t0 + t < depth;
-      sa[t][i] = live && i0 + i < rows ? a(t0 + t, i0 + i) : 0.f;
-      sb[t][i] = live && j0 + i < cols ? b(t0 + t, j0 + i) : 0.f;
+struct Fp4Args {
+  const uint8_t* a_scales;
+  const uint8_t* b_scales;
+  int k_padded, steps, ktiles, splits;
+  int n_tiles, m_tiles;
+  OutMatrix out;
+};
+
+template <int BN>
+__global__ void __launch_bounds__(kTcThreads, 2)
+mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp4Args a) {
+  using S = Fp4Smem<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t tile_b = base, tile_a = tile_b + S::kStages * S::kA, scale_b = tile_a + S::kStages * S::kB;   // b's rows are the lanes
+  const uint32_t scale_a = scale_b + S::kStages * S::kScale, bars = scale_a + S::kStages * S::kScale;
+  const uint32_t full = bars, empty = bars + 8 * S::kStages, done = empty + 8 * S::kStages, slot = done + 8;
+  const int warp = threadIdx.x >> 5;
+
+  const int tile = blockIdx.x / a.splits, rank = blockIdx.x % a.splits;
+  const int per_group = 8 * a.n_tiles, group = tile / per_group, width = min(8, a.m_tiles - 8 * group);
+  const int in_group = tile - group * per_group;
+  const int m0 = (group * 8 + in_group % width) * BN, nt = in_group / width, n0 = nt * 128;
+  const int first = (int)((int64_t)a.steps * rank / a.splits), last = (int)((int64_t)a.steps * (rank + 1) / a.splits);
+
+  if (warp == 0 && elect_one()) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
     }
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < 16; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[t][ti + 16 * i], sb[t][tj + 16 * j], acc[i][j]);
-    __syncthreads();
+    mbar_init(done, 1);
+    fence_barrier_init();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t r = i0 + ti + 16 * i, c = j0 + tj + 16 * j;
-      if (r >= rows || c >= cols) continue;
-      const int64_t at = r * ld + c;
-      if (out_dtype == RT_F32) {
-        float* o = static_cast<float*>(out) + at;
-        *o = accumulate ? *o + acc[i][j] : acc[i][j];
-      } else {
-        uint16_t* o = static_cast<uint16_t*>(out) + at;
-        if (out_dtype == RT_BF16) *o = of_f32<RT_BF16>(accumulate ? to_f32<RT_BF16>(*o) + acc[i][j] : acc[i][j]);
-        else *o = of_f32<RT_F16>(accumulate ? to_f32<RT_F16>(*o) + acc[i][j] : acc[i][j]);
+  if (warp == 2) tmem_alloc(slot, S::kColumns);
+  __syncthreads();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
+  bool ok = true;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint8_t* sb = a.b_scales + (int64_t)nt * a.ktiles * 512;
+      const uint8_t* sa = a.a_scales + (int64_t)(m0 >> 7) * a.ktiles * 512;
+      int i = 0;
+      for (int it = first; it < last; ++it, ++i) {
+        const int s = i % S::kStages;
+        if (!(ok = mbar_wait(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
+        const uint32_t bytes = 512u * min(2, a.ktiles - 2 * it);
+        mbar_expect(full + 8 * s, S::kA + S::kB + 2 * bytes);
+        tma_load_2d(&map_b, tile_b + s * S::kA, full + 8 * s, it * 128, n0);
+        tma_load_2d(&map_a, tile_a + s * S::kB, full + 8 * s, it * 128, m0);
+        bulk_load(scale_b + s * S::kScale, sb + (int64_t)it * 1024, bytes, full + 8 * s);
+        bulk_load(scale_a + s * S::kScale, sa + (int64_t)it * 1024, bytes, full + 8 * s);
       }
+      if (!ok)   // the loads in flight still write to this CTA's memory
+        for (int j = 0; j < S::kStages && j < i; ++j) {
+          const int latest = i - 1 - (i - 1 - j) % S::kStages;
+          mbar_wait(full + 8 * j, (latest / S::kStages) & 1);
+        }
     }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      for (int i = 0; i < last - first; ++i) {
+        const int s = i % S::kStages, it = first + i;
+        if (!(ok = mbar_wait(full + 8 * s, (i / S::kStages) & 1))) break;
+        tc_fence_after();
+        const uint32_t sf = tmem + BN + 16 * s;
+        const int halves = min(2, a.ktiles - 2 * it), products = min(4, (a.k_padded - it * kStepK + 63) / 64);
+        for (int h = 0; h < halves; ++h) {
+          copy_scales(sf + 4 * h, plain_desc(scale_b + s * S::kScale + 512 * h, 128, 128));
+          copy_scales(sf + 8 + 4 * h, plain_desc(scale_a + s * S::kScale + 512 * h, 128, 128));
+        }
+        const uint64_t db = tile_desc(tile_b + s * S::kA, 16, 1024), da = tile_desc(tile_a + s * S::kB, 16, 1024);
+        for (int kk = 0; kk < products; ++kk)
+          mma_mxfp4(tmem, db + kk * 2, da + kk * 2, kk & 1 ? idesc_mxfp4(128, BN, 1) : idesc_mxfp4(128, BN, 0), sf + 4 * (kk >> 1),
+                    sf + 8 + 4 * (kk >> 1), i > 0 || kk > 0);
+        tc_commit(empty + 8 * s);
+      }
+      tc_commit(done);
+    }
+  } else if (warp >= kFirstWorker) {
+    ok = mbar_wait(done, 0);
+    tc_fence_after();
+  }
+  __syncwarp();
+  if (!ok) atomicAdd(&g_wait_faults, 1u);
+  finish_tile<BN>(a.out, tmem, m0, n0, a.splits, reinterpret_cast<float*>(smem), ok);
+  __syncthreads();
+  if (warp == 2) tmem_free(tmem, S::kColumns);
 }
 
 static int check_out(const void* out, int dtype, int64_t cols, int64_t ld) {
@@ -419,6 +479,12 @@ template <int BN>
 static int run_wgrad(const CUtensorMap& codes, const CUtensorMap& grad, const WgradArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
   return launch_tc(mx_weight_grad_kernel<BN>, raised, WgradSmem<BN>::kBytes, (int64_t)a.k_tiles * a.n_tiles * a.splits, a.splits, st, codes, grad, a);
+}
+
+template <int BN>
+static int run_fp4(const CUtensorMap& ma, const CUtensorMap& mb, const Fp4Args& a, cudaStream_t st) {
+  static std::atomic<uint64_t> raised{0};
+  return launch_tc(mx_fp4_kernel<BN>, raised, Fp4Smem<BN>::kBytes, (int64_t)a.n_tiles * a.m_tiles * a.splits, a.splits, st, ma, mb, a);
 }
 
 static int pieces_of(int dtype) { return dtype == RT_F32 ? 3 : dtype == RT_F16 ? 2 : 1; }
@@ -528,15 +594,52 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
   if (int rc = mx_check_shape(n, k)) return rc;
   if (m == 0 || n == 0) return 0;
   if (int rc = check_out(out, out_dtype, n, ld_out)) return rc;
-  if (k > 0) {
-    if (int rc = mx_check_codes(a_codes, a_scales)) return rc;
-    if (int rc = mx_check_codes(b_codes, b_scales)) return rc;
+  cudaStream_t st = (cudaStream_t)cuda_stream;
+  if (k == 0) {                             // an empty sum
+    const size_t size = dtype_size(out_dtype);
+    RT_CUDA(cudaMemset2DAsync(out, ld_out * size, 0, n * size, m, st));
+    return 0;
   }
+  if (int rc = mx_check_codes(a_codes, a_scales)) return rc;
+  if (int rc = mx_check_codes(b_codes, b_scales)) return rc;
   const int64_t kp = pad_to(k, kMxBlock);
-  const int kt = (int)((kp + 127) / 128);
-  const FromFp4 a{(const uint8_t*)a_codes, (const uint8_t*)a_scales, kp / 2, kt}, b{(const uint8_t*)b_codes, (const uint8_t*)b_scales, kp / 2, kt};
-  const dim3 grid((unsigned)((n + 63) / 64), (unsigned)((m + 63) / 64));
-  if (grid.y > 65535) return fail(RT_E_SIZE, "m too large");
-  simple_product_kernel<<<grid, 256, 0, (cudaStream_t)cuda_stream>>>(a, b, k, m, n, out, out_dtype, ld_out, 0);
-  return launched();
+  Fp4Args a{};
+  a.a_scales = (const uint8_t*)a_scales;
+  a.b_scales = (const uint8_t*)b_scales;
+  a.k_padded = (int)kp;
+  a.steps = (int)((kp + kStepK - 1) / kStepK);
+  a.ktiles = (int)((kp + 127) / 128);
+  a.out = {out, ld_out, (int)m, (int)n, out_dtype, 0};
+
+  const int64_t n_tiles = (n + 127) / 128;
+  int bm = 128, splits = 1;
+  double best = 1e300;
+  for (const int width : {128, 64, 32})
+    for (const int s : {1, 2, 4, 8}) {
+      if (s > a.steps || (width < 128 && m > width)) continue;
+      const double step = width == 128 ? 450 : width == 64 ? 300 : 250;
+      const int64_t ctas = n_tiles * ((m + width - 1) / width) * s;
+      const double cost = (double)((ctas + 2 * kSms - 1) / (2 * kSms)) * ((double)((a.steps + s - 1) / s) * step + 2000 + width * 12 + (s > 1 ? 1500 : 0));
+      if (cost < best) { best = cost; bm = width; splits = s; }
+    }
+  a.splits = splits;
+  a.n_tiles = (int)n_tiles;
+  a.m_tiles = (int)((m + bm - 1) / bm);
+  if (n_tiles * a.m_tiles * splits > 0x7FFFFFFFll) return fail(RT_E_SIZE, "m * n is too large");
+
+  CUtensorMap map_a, map_b;
+  const uint64_t strides[1] = {(uint64_t)kp / 2};
+  {
+    const uint64_t dims[2] = {(uint64_t)kp / 2, (uint64_t)m};
+    const uint32_t box[2] = {128, (uint32_t)bm};
+    if (int rc = make_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  {
+    const uint64_t dims[2] = {(uint64_t)kp / 2, (uint64_t)n};
+    const uint32_t box[2] = {128, 128};
+    if (int rc = make_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, b_codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  if (bm == 128) return run_fp4<128>(map_a, map_b, a, st);
+  if (bm == 64) return run_fp4<64>(map_a, map_b, a, st);
+  return run_fp4<32>(map_a, map_b, a, st);
 }
