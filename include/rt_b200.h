@@ -347,7 +347,7 @@ int rt_host_unregister(void* ptr);
  *              mantissa bit of y = x * 2^-e on the grid 0, .5, 1, 1.5, 2, 3, 4, 6 (two codes per
  *              byte, the even column in the low half); value = grid value * 2^e
  *              nearest: ties to the even mantissa bit; stochastic: floor(|y| / s + r16 / 65536) * s,
- *              s the grid's step at |y| (0.5 below 2, 1 below 4, else 2)
+ *              s the grid's step at |y| (0.5 below 2, 1 below 4, else 2), a zero being +0
  *   a block with an infinity or a NaN: scale byte 255, codes 0; its values read as NaN.
  * Nothing saturates except at the top of the range: MXINT8 at 127 * 2^121, MXFP4 (e = 126) at
  * 3 * 2^126, so that what is finite stays finite.  Every value is exactly a

@@ -4,10 +4,12 @@
 //
 // All of it is bound by memory: each value is read once and written once, 32 values share one
 // reduction of four lanes.  A thread handles UNITS of eight consecutive values of a row (16 bytes
-// of bf16 per access); the units of a matrix are numbered row by row over rows padded to whole
-// blocks, so the four lanes of a block are always neighbours in a warp, whatever the row length.
-// Rows that do not start on 16-byte boundaries go through a warp's slice of shared memory, so
-// that global accesses stay consecutive; the arithmetic after it is the same.
+// of bf16 per access), the same unit of two or four consecutive rows: it works out once where that is,
+// and has all its loads under way before it uses the first.  Neighbouring threads have neighbouring
+// units of rows padded to whole blocks, so a block's four lanes are neighbours whatever the row length.
+// Rows that do not start on 16-byte boundaries are read and written as aligned 16-byte chunks all the
+// same: a unit is cut out of two neighbouring chunks, an output chunk is put together from two
+// neighbouring lanes' units; only the ends of a row go value by value.
 #include <algorithm>
 
 #include "mx_common.cuh"
@@ -16,164 +18,253 @@
 namespace rt {
 
 constexpr int kMxThreads = 256;
-constexpr int kMxWarps = kMxThreads / 32;
 constexpr uint32_t kStreamFp4 = 3;  // Philox counter word 3 of the 4-bit rounding
 
 struct Matrix {            // rows x cols, row stride ld elements
   const void* p;
   int64_t ld;
 };
-struct Grid {              // how the units of a matrix are numbered
+struct Grid {              // how the units of a matrix are handed out
   FastDiv upr;             // units per row
-  uint32_t units;
   int cols;
   uint32_t rows;
 };
+// A thread's units: unit c8 of rows r .. r + R - 1
+template <int R>
+struct Place {
+  uint32_t r, c8;
+  int c;
+  __device__ __forceinline__ explicit Place(const Grid& g) {
+    uint32_t group;
+    g.upr.split(blockIdx.x * kMxThreads + threadIdx.x, group, c8);
+    r = group * R;
+    c = (int)c8 * 8;
+  }
+  __device__ __forceinline__ bool live(const Grid& g, int k) const { return r + k < g.rows; }
+  __device__ __forceinline__ uint32_t unit(const Grid& g, int k) const { return (r + k) * g.upr.d + c8; }
+};
 
 // ---------------------------------------------------------------------------------------- units
-// Unit -> eight fp32 values; columns beyond the last are 0.  `stage`: 256 floats of this warp.
+// the 16 bytes from byte `off` (even, below 16) of the 32 bytes a, b
+__device__ __forceinline__ uint4 cut16(const uint4& a, const uint4& b, uint32_t off) {
+  const bool two = off & 8u, one = off & 4u;
+  const uint32_t t0 = two ? a.z : a.x, t1 = two ? a.w : a.y, t2 = two ? b.x : a.z, t3 = two ? b.y : a.w, t4 = two ? b.z : b.x, t5 = two ? b.w : b.y;
+  const uint32_t v0 = one ? t1 : t0, v1 = one ? t2 : t1, v2 = one ? t3 : t2, v3 = one ? t4 : t3, v4 = one ? t5 : t4;
+  const uint32_t sh = (off & 3u) * 8;
+  return make_uint4(__funnelshift_r(v0, v1, sh), __funnelshift_r(v1, v2, sh), __funnelshift_r(v2, v3, sh), __funnelshift_r(v3, v4, sh));
+}
+
+// The unit at p, column c of its row; columns beyond the last are 0.  VEC: every row starts on a
+// 16-byte boundary.  Otherwise a unit that has a whole unit before it and 16 bytes of its row behind
+// it is cut out of aligned chunks, which then lie inside the row.
 template <int D, bool VEC>
-__device__ __forceinline__ void load_staged(const Matrix& m, const Grid& g, uint32_t warp_unit, int lane, float* stage, float (&x)[8]) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t u = warp_unit + 4 * j + (lane >> 3);
-    float v = 0.f;
-    if (u < g.units) {
-      uint32_t r, c;
-      g.upr.split(u, r, c);
-      c = c * 8 + (lane & 7);
-      if ((int)c < g.cols) v = to_f32<D>(static_cast<const elem_t<D>*>(m.p)[(int64_t)r * m.ld + c]);
-    }
-    stage[j * 32 + lane] = v;
-  }
-  __syncwarp();
-  const float4 a = reinterpret_cast<const float4*>(stage)[lane * 2], b = reinterpret_cast<const float4*>(stage)[lane * 2 + 1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  __syncwarp();
-}
-template <int D>
-__device__ __forceinline__ void store_staged(const Matrix& m, const Grid& g, uint32_t warp_unit, int lane, float* stage, const float (&x)[8]) {
-  reinterpret_cast<float4*>(stage)[lane * 2] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(stage)[lane * 2 + 1] = make_float4(x[4], x[5], x[6], x[7]);
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t u = warp_unit + 4 * j + (lane >> 3);
-    if (u < g.units) {
-      uint32_t r, c;
-      g.upr.split(u, r, c);
-      c = c * 8 + (lane & 7);
-      if ((int)c < g.cols) static_cast<elem_t<D>*>(const_cast<void*>(m.p))[(int64_t)r * m.ld + c] = of_f32<D>(stage[j * 32 + lane]);
-    }
-  }
-  __syncwarp();
-}
-// VEC: rows start on 16-byte boundaries; only a row's last unit may be cut
-template <int D>
-__device__ __forceinline__ Raw8<D> load_unit(const Matrix& m, const Grid& g, uint32_t r, uint32_t c8, bool live) {
+__device__ __forceinline__ Raw8<D> load_unit(const elem_t<D>* p, const int c, const int cols, const bool live) {
+  constexpr int kSize = sizeof(elem_t<D>);
   Raw8<D> raw{};
-  const int c = (int)c8 * 8;
-  if (live && c + 8 <= g.cols) raw = load_raw<D>(m.p, (int64_t)r * m.ld + c);
-  else if (live && c < g.cols) {
+  if (!live) return raw;
+  const uint32_t off = VEC ? 0u : (uint32_t)(uintptr_t)p & 15u;
+  if ((VEC || off == 0) && c + 8 <= cols) {
+    raw = load_raw<D>(p, 0);
+  } else if (!VEC && c >= 8 && c + 8 + 16 / kSize <= cols) {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+    const uint4 a = __ldg(q), b = __ldg(q + 1);
+    raw.w[0] = cut16(a, b, off);
+    if constexpr (D == RT_F32) raw.w[1] = cut16(b, __ldg(q + 2), off);
+  } else if (c < cols) {
     float x[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = c + k < g.cols ? to_f32<D>(static_cast<const elem_t<D>*>(m.p)[(int64_t)r * m.ld + c + k]) : 0.f;
+    for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? to_f32<D>(p[k]) : 0.f;
     raw = pack<D>(x);   // exact: the values are of this type
   }
   return raw;
 }
-template <int D>
-__device__ __forceinline__ void store_unit(const Matrix& m, const Grid& g, uint32_t r, uint32_t c8, const float (&x)[8]) {
-  const int c = (int)c8 * 8;
-  void* p = const_cast<void*>(m.p);
-  if (c + 8 <= g.cols) store_raw<D>(p, (int64_t)r * m.ld + c, pack<D>(x));
-  else {
+// the units of a thread; rows step rows apart
+template <int D, bool VEC, int R>
+__device__ __forceinline__ void load_units(const Matrix& m, int64_t row, int step, int c, int cols, int64_t rows, Raw8<D> (&raw)[R]) {
+  const elem_t<D>* p = static_cast<const elem_t<D>*>(m.p) + row * m.ld + c;
+  if (VEC && c + 8 <= cols && row + (R - 1) * step < rows) {      // nearly always: nothing to look at again
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < g.cols) static_cast<elem_t<D>*>(p)[(int64_t)r * m.ld + c + k] = of_f32<D>(x[k]);
+    for (int k = 0; k < R; ++k) raw[k] = load_raw<D>(p, k * step * m.ld);
+  } else {
+#pragma unroll
+    for (int k = 0; k < R; ++k) raw[k] = load_unit<D, VEC>(p + k * step * m.ld, c, cols, row + k * step < rows);
+  }
+}
+template <int D>
+__device__ __forceinline__ void store_each(elem_t<D>* p, const float (&x)[8], int from, int to) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k >= from && k < to) p[k] = of_f32<D>(x[k]);
+}
+// All lanes of a warp call this together: lane l holds the unit after lane l - 1's.
+template <int D, bool VEC>
+__device__ __forceinline__ void store_unit(const Matrix& m, const int cols, uint32_t r, const int c, bool live, const float (&x)[8]) {
+  constexpr int kSize = sizeof(elem_t<D>);
+  elem_t<D>* p = static_cast<elem_t<D>*>(const_cast<void*>(m.p)) + (int64_t)r * m.ld + c;
+  if constexpr (VEC) {
+    if (live && c + 8 <= cols) store_raw<D>(p, 0, pack<D>(x));
+    else if (live) store_each<D>(p, x, 0, cols - c);
+  } else {
+    const Raw8<D> own = pack<D>(x);
+    const uint4 last = own.w[D == RT_F32 ? 1 : 0];
+    uint4 before;
+    before.x = __shfl_up_sync(0xFFFFFFFFu, last.x, 1);
+    before.y = __shfl_up_sync(0xFFFFFFFFu, last.y, 1);
+    before.z = __shfl_up_sync(0xFFFFFFFFu, last.z, 1);
+    before.w = __shfl_up_sync(0xFFFFFFFFu, last.w, 1);
+    if (!live) return;
+    const int lane = threadIdx.x & 31;
+    const uint32_t off = (uint32_t)(uintptr_t)p & 15u;
+    if (c + 8 > cols) store_each<D>(p, x, 0, cols - c);
+    else if (off == 0) store_raw<D>(p, 0, own);
+    else {
+      // chunk 0 holds the lane before's last `off` bytes and this unit's first; the last `off` bytes here go with the next lane's
+      uint4* q = reinterpret_cast<uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+      const int head = (int)(16u - off) / kSize, tail = 8 - (int)off / kSize;
+      if (lane > 0 && c > 0) q[0] = cut16(before, own.w[0], 16u - off);
+      else store_each<D>(p, x, 0, head);
+      if constexpr (D == RT_F32) q[1] = cut16(own.w[0], own.w[1], 16u - off);
+      if (lane == 31 || c + 16 > cols) store_each<D>(p, x, tail, 8);
+    }
   }
 }
 
 // -------------------------------------------------------------------------------------- formats
-// The largest magnitude of a block as a bit pattern: integer order is the order of magnitudes, with
-// infinities and NaNs on top, so one maximum also finds the blocks that hold any.
-__device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
-  uint32_t a = 0;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) a = max(a, __float_as_uint(x[k]) & 0x7FFFFFFFu);
-  return a;
+// The largest magnitude of a block as an fp32 bit pattern: integer order is the order of
+// magnitudes, with infinities and NaNs on top, so one maximum also finds the blocks that hold any.
+// 16-bit types take two values per instruction until the end.
+template <int D>
+__device__ __forceinline__ uint32_t amax_words(const uint4& w) {
+  if constexpr (D == RT_F32) return max(max(w.x & 0x7FFFFFFFu, w.y & 0x7FFFFFFFu), max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu));
+  else return __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu));
 }
-__device__ __forceinline__ uint32_t amax_of_four(uint32_t a) {
-  a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1));
-  return max(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2));
+template <int D>
+__device__ __forceinline__ uint32_t amax_both(uint32_t a, uint32_t b) { return D == RT_F32 ? max(a, b) : __vmaxu2(a, b); }
+template <int D>
+__device__ __forceinline__ uint32_t amax_bits(uint32_t a) {
+  if constexpr (D == RT_F32) return a;
+  a = max(a & 0xFFFFu, a >> 16);
+  return D == RT_BF16 ? a << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)a)));
+}
+template <int D>
+__device__ __forceinline__ uint32_t amax_of_block(const Raw8<D>& raw) {   // four neighbouring lanes hold the block
+  uint32_t a = amax_words<D>(raw.w[0]);
+  if constexpr (D == RT_F32) a = max(a, amax_words<D>(raw.w[1]));
+  a = amax_both<D>(a, __shfl_xor_sync(0xFFFFFFFFu, a, 1));
+  return amax_bits<D>(amax_both<D>(a, __shfl_xor_sync(0xFFFFFFFFu, a, 2)));
 }
 
-// Eight MXINT8 codes.  x * 2^(6-e) is exact; adding 1.5 * 2^23 rounds it to an integer, ties to
-// even, and leaves that integer's two's complement in the low bits.
+// packed fp32 arithmetic: two IEEE operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2_rz(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rz.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// Eight MXINT8 codes of each lane's block.  x * 2^(6-e) is exact; adding 1.5 * 2^23 in the same
+// operation rounds it to an integer, ties to even, and leaves that integer's two's complement in the
+// low bits.  Only the topmost magnitudes can reach 128; those and what is not finite are looked
+// after in a branch that a warp hardly ever takes.  All lanes call it together.
 __device__ __forceinline__ uint2 codes_int8(const float (&x)[8], uint32_t amax, uint32_t& byte) {
-  const bool bad = amax >= 0x7F800000u;
-  const int e = exponent_int8(amax);
-  byte = bad ? 255u : (uint32_t)(e + 127);
-  const float s = pow2f(6 - e);
+  byte = byte_of_int8(amax);
+  const float s = __uint_as_float((260u - byte) << 23);
+  const float2 ss = make_float2(s, s), magic = make_float2(12582912.f, 12582912.f);
   uint32_t q[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) q[k] = __float_as_uint(fminf(fmaxf(x[k] * s, -127.f), 127.f) + 12582912.f);
+  for (int k = 0; k < 4; ++k) {
+    const float2 r = fma2(make_float2(x[2 * k], x[2 * k + 1]), ss, magic);
+    q[2 * k] = __float_as_uint(r.x);
+    q[2 * k + 1] = __float_as_uint(r.y);
+  }
+  const bool top = amax > 0x7F7E0000u;             // above 127 * 2^121, infinities and NaNs among them
+  if (__any_sync(0xFFFFFFFFu, top)) {
+    const bool bad = amax >= 0x7F800000u;
+    if (bad) byte = 255u;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (top) q[k] = bad ? 0u : __float_as_uint(fminf(fmaxf(x[k] * s, -127.f), 127.f) + 12582912.f);
+  }
   uint2 w;
   w.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
   w.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
-  return bad ? make_uint2(0u, 0u) : w;
+  return w;
 }
 
-// two values, the second in the low half of the byte; nearest, ties to even
-__device__ __forceinline__ uint32_t cvt_e2m1x2(float high, float low) {
+// eight values, already on the grid's scale, to codes: nearest, ties to even, the even value in the low half of a byte
+__device__ __forceinline__ uint32_t cvt_e2m1x8(const float (&y)[8]) {
   uint32_t r;
-  asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(high), "f"(low));
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return r;
 }
-// Stochastic rounding to the grid: floor(|y|/s + r/65536) * s with s the grid's step at |y| (0.5
-// below 2, 1 below 4, else 2).  From 1 upwards that is an integer addition to the bit pattern, one
-// mantissa bit kept; below 1 the same holds for |y| + 1, whose step is 0.5 too (added towards zero:
-// what is cut off lies below the last place that the comparison with r can see).
-__device__ __forceinline__ float sr_e2m1(float y, uint32_t r16) {
-  const uint32_t sign = __float_as_uint(y) & 0x80000000u;
-  const float a = fabsf(y);
-  const float one = a < 1.f ? 1.f : 0.f;
-  const float b = __fadd_rz(a, one);
-  const float v = __uint_as_float((__float_as_uint(b) + (r16 << 6)) & 0xFFC00000u) - one;
-  return __uint_as_float(__float_as_uint(v) | sign);
+// Stochastic rounding of two values to the grid: floor(|y|/s + r/65536) * s with s the grid's step
+// at |y| (0.5 below 2, 1 below 4, else 2).  From 1 upwards that is an integer addition of r * 64 to the
+// bit pattern, one mantissa bit kept, whatever the sign; below 1 the same holds for |y| + 1, whose step
+// is 0.5 too (added towards zero: what is cut off lies below the last place that r can reach).
+// A zero that comes of this is +0.
+__device__ __forceinline__ void sr_pair(float2 y, uint32_t draws, float& y0, float& y1) {
+  const float t0 = fabsf(y.x) < 1.f ? 1.f : 0.f, t1 = fabsf(y.y) < 1.f ? 1.f : 0.f;
+  const float2 t = make_float2(__uint_as_float(__float_as_uint(t0) | (__float_as_uint(y.x) & 0x80000000u)),
+                               __uint_as_float(__float_as_uint(t1) | (__float_as_uint(y.y) & 0x80000000u)));
+  const float2 b = add2_rz(y, t);
+  const uint32_t u = ((draws & 0xFFFFu) * 64u + __float_as_uint(b.x)) & 0xFFC00000u, v = ((draws >> 16) * 64u + __float_as_uint(b.y)) & 0xFFC00000u;
+  const float2 c = fma2(t, make_float2(-1.f, -1.f), make_float2(__uint_as_float(u), __uint_as_float(v)));
+  y0 = c.x;
+  y1 = c.y;
 }
-// Eight MXFP4 codes, the even value in the low half of a byte.
+__device__ __forceinline__ uint32_t byte_fp4(uint32_t amax) { return amax >= 0x7F800000u ? 255u : byte_of_fp4(amax); }
+// Eight MXFP4 codes of a block whose scale byte is known (255: not finite).  All lanes that are here together vote.
 template <bool SR>
-__device__ __forceinline__ uint32_t codes_fp4(const float (&x)[8], uint32_t amax, uint32_t& byte, const PhiloxKeys& keys,
-                                              uint32_t tensor_id, uint32_t step, uint32_t unit) {
-  const bool bad = amax >= 0x7F800000u;
-  const int e = exponent_fp4(amax);
-  byte = bad ? 255u : (uint32_t)(e + 127);
-  const float s = pow2f(-e);
-  float y[8];
+__device__ __forceinline__ uint32_t codes_fp4(const float (&x)[8], uint32_t byte, const PhiloxKeys& keys, uint32_t tensor_id, uint32_t step, uint32_t unit) {
+  const float s = pow2f(127 - (int)byte);
+  const float2 ss = make_float2(s, s);
+  float2 p[4];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) y[k] = x[k] * s;
-  if (e == 126) {                     // 4 * 2^126 is no fp32 number: what is finite stays finite
+  for (int k = 0; k < 4; ++k) p[k] = mul2(make_float2(x[2 * k], x[2 * k + 1]), ss);
+  if (__any_sync(__activemask(), byte >= 253u)) {   // 253: 4 * 2^126 is no fp32 number, what is finite stays finite; 255: codes 0
+    const float top = byte == 255u ? 0.f : byte == 253u ? 3.f : 6.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = fminf(fmaxf(y[k], -3.f), 3.f);
+    for (int k = 0; k < 4; ++k) p[k] = make_float2(fminf(fmaxf(p[k].x, -top), top), fminf(fmaxf(p[k].y, -top), top));
   }
+  float y[8];
   if constexpr (SR) {
     const uint4 d = draws8(keys, tensor_id, step, kStreamFp4, unit);
-    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+    sr_pair(p[0], d.x, y[0], y[1]);
+    sr_pair(p[1], d.y, y[2], y[3]);
+    sr_pair(p[2], d.z, y[4], y[5]);
+    sr_pair(p[3], d.w, y[6], y[7]);
+  } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = sr_e2m1(y[k], k & 1 ? w[k >> 1] >> 16 : w[k >> 1] & 0xFFFFu);
+    for (int k = 0; k < 4; ++k) { y[2 * k] = p[k].x; y[2 * k + 1] = p[k].y; }
   }
-  uint32_t c = 0;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) c |= cvt_e2m1x2(y[2 * k + 1], y[2 * k]) << (8 * k);
-  return bad ? 0u : c;
+  const uint32_t c = cvt_e2m1x8(y);
+  return byte == 255u ? 0u : c;
 }
 // Eight values of MXINT8 codes.  The byte with its sign turned over, set into the mantissa of 2^23, is 2^23 + 128 + code.
 __device__ __forceinline__ void values_int8(uint2 w, float s, float (&x)[8]) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const uint32_t u = (k < 4 ? w.x : w.y) ^ 0x80808080u;
-    x[k] = (__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | (k & 3))) - 8388736.f) * s;
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t u = (k < 2 ? w.x : w.y) ^ 0x80808080u;
+    const float2 f = make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | ((2 * k) & 3))),
+                                 __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | ((2 * k + 1) & 3))));
+    const float2 v = mul2(add2_rz(f, make_float2(-8388736.f, -8388736.f)), make_float2(s, s));   // the sum is exact
+    x[2 * k] = v.x;
+    x[2 * k + 1] = v.y;
   }
 }
 // Eight values of MXFP4 codes: exponent and mantissa bits of a code, moved to bit 22, times 2^126.
@@ -186,21 +277,24 @@ __device__ __forceinline__ void values_fp4(uint32_t w, float s, float (&x)[8]) {
   }
 }
 
-__device__ __forceinline__ void put_int8(uint8_t* codes, uint8_t* scales, const Grid& g, uint32_t r, uint32_t c8, uint2 w, uint32_t byte) {
-  *reinterpret_cast<uint2*>(codes + ((int64_t)r * g.upr.d + c8) * 8) = w;
-  if ((c8 & 3) == 0) {
-    const int nb = g.upr.d >> 2, stride = (nb + 3) & ~3, b = c8 >> 2;
-    uint8_t* row = scales + (int64_t)r * stride;
-    row[b] = (uint8_t)byte;
-    if (b == nb - 1)
-      for (int k = nb; k < stride; ++k) row[k] = 0;
-  }
+// where a thread's first scale byte goes; the byte of the next row is `stride` further
+template <int R>
+__device__ __forceinline__ uint8_t* int8_scale(uint8_t* scales, const Grid& g, const Place<R>& at, int& stride) {
+  stride = ((g.upr.d >> 2) + 3) & ~3u;
+  return scales + (int64_t)at.r * stride + (at.c8 >> 2);
 }
-__device__ __forceinline__ void put_fp4_scale(uint8_t* scales, int nb, int64_t r, int b, uint32_t byte) {
-  const int ktiles = (nb + 3) >> 2;
-  scales[fp4_scale_at(r, b, ktiles)] = (uint8_t)byte;
+// one lane of a block stores its scale, the last block's also the zeros that fill the row
+__device__ __forceinline__ void put_int8_scale(uint8_t* p, int nb, uint32_t c8, uint32_t byte) {
+  if ((c8 & 3) != 0) return;
+  *p = (uint8_t)byte;
+  if ((int)(c8 >> 2) == nb - 1)
+    for (int k = nb; k & 3; ++k) p[k - nb + 1] = 0;
+}
+// the four blocks of a tile's row are neighbours, so the same holds here
+__device__ __forceinline__ void put_fp4_scale(uint8_t* p, int nb, int b, uint32_t byte) {
+  *p = (uint8_t)byte;
   if (b == nb - 1)
-    for (int k = nb; k < 4 * ktiles; ++k) scales[fp4_scale_at(r, k, ktiles)] = 0;
+    for (int k = nb; k & 3; ++k) p[k - nb + 1] = 0;
 }
 // the scale bytes of the rows that fill the last tile of 128
 __device__ __forceinline__ void clear_fp4_pad(uint8_t* scales, uint32_t rows, int nb, uint32_t tid, uint32_t threads) {
@@ -216,107 +310,109 @@ struct SrArgs {
 };
 
 // ------------------------------------------------------------------------------------- quantise
-// FMT 0: MXINT8, 1: MXFP4.  A CTA takes kUnits units per thread and loads them all before the
-// first is used.
-constexpr int kUnits = 4;
+// FMT 0: MXINT8, 1: MXFP4.
+constexpr int kRows = 4;   // rows to a thread
 
 template <int D, int FMT, bool SR, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
 mx_quantize_kernel(const Matrix x, const Grid g, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const SrArgs sr) {
-  __shared__ float stage[VEC ? 1 : kMxWarps * 256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t first = blockIdx.x * (kMxThreads * kUnits) + threadIdx.x;
-  Raw8<D> raw[VEC ? kUnits : 1];
-  if constexpr (VEC) {
+  const Place<kRows> at(g);
+  const int nb = g.upr.d >> 2;
+  Raw8<D> raw[kRows];
+  load_units<D, VEC>(x, at.r, 1, at.c, g.cols, g.rows, raw);
+  int stride;
+  uint8_t* sp;
+  if constexpr (FMT == RT_MXINT8) sp = int8_scale(scales, g, at, stride);
+  else { sp = scales + fp4_scale_at(at.r, at.c8 >> 2, (nb + 3) >> 2); stride = 16; }   // four rows from a multiple of four: one tile, one group
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const uint32_t u = first + k * kMxThreads;
-      uint32_t r, c;
-      g.upr.split(u, r, c);
-      raw[k] = load_unit<D>(x, g, r, c, u < g.units);
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    const uint32_t u = first + k * kMxThreads;
+  for (int k = 0; k < kRows; ++k) {
+    const uint32_t u = at.unit(g, k), amax = amax_of_block<D>(raw[k]);
     float v[8];
-    if constexpr (VEC) unpack<D>(raw[k], v);
-    else load_staged<D, VEC>(x, g, u - lane, lane, stage + warp * 256, v);
-    const uint32_t amax = amax_of_four(amax8(v));
-    uint32_t r, c, byte;
-    g.upr.split(u, r, c);
+    unpack<D>(raw[k], v);
     if constexpr (FMT == RT_MXINT8) {
+      uint32_t byte;
       const uint2 w = codes_int8(v, amax, byte);
-      if (u < g.units) put_int8(codes, scales, g, r, c, w, byte);
+      if (at.live(g, k)) {
+        reinterpret_cast<uint2*>(codes)[u] = w;
+        put_int8_scale(sp + k * stride, nb, at.c8, byte);
+      }
     } else {
-      const uint32_t w = codes_fp4<SR>(v, amax, byte, sr.keys, sr.tensor_id, sr.step, u);
-      if (u < g.units) {
+      const uint32_t byte = byte_fp4(amax), w = codes_fp4<SR>(v, byte, sr.keys, sr.tensor_id, sr.step, u);
+      if (at.live(g, k)) {
         reinterpret_cast<uint32_t*>(codes)[u] = w;
-        if ((c & 3) == 0) put_fp4_scale(scales, g.upr.d >> 2, r, c >> 2, byte);
+        if ((at.c8 & 3) == 0) put_fp4_scale(sp + k * stride, nb, at.c8 >> 2, byte);
       }
     }
   }
-  if constexpr (FMT == RT_MXFP4)
-    clear_fp4_pad(scales, g.rows, g.upr.d >> 2, blockIdx.x * kMxThreads + threadIdx.x, gridDim.x * kMxThreads);
+  if constexpr (FMT == RT_MXFP4) clear_fp4_pad(scales, g.rows, nb, blockIdx.x * kMxThreads + threadIdx.x, gridDim.x * kMxThreads);
 }
 
 // ------------------------------------------------------------------------- quantise, transposed
-// Output row c holds column c of x, in blocks along x's rows.  A CTA takes 128 rows x 64 columns
-// through shared memory; thread (column, quarter) then owns one block of 32 rows, so that the
-// block's maximum needs no exchange.
-constexpr int kTRows = 128, kTCols = 64;
+// Output row c holds column c of x, in blocks along x's rows.  A CTA takes 128 rows x 256 bytes
+// through shared memory.  A thread then owns one 4-byte column (two columns of a 16-bit type) of 32
+// rows, that is one or two whole blocks, so a block's maximum needs no exchange.  Eight
+// neighbouring columns x four blocks make a warp: an output row's four blocks (64 bytes) are
+// stored together.  The 32-byte pieces of a row are exchanged by the row's group of 32 (bits 3 and 4 of
+// the word index), which keeps those four lanes' reads in different banks.
+constexpr int kTRows = 128, kTWords = 64;
 
 template <int D, bool SR, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, 4)
 mx_quantize_t_kernel(const Matrix x, const int64_t rows, const int cols, const uint32_t col_tiles, uint8_t* __restrict__ codes,
                      uint8_t* __restrict__ scales, const SrArgs sr) {
-  using T = elem_t<D>;
-  __shared__ __align__(16) T tile[kTRows][kTCols];
+  constexpr int kPer = D == RT_F32 ? 1 : 2;             // columns to a word
+  constexpr int kTCols = kTWords * kPer, kUnitsPerRow = kTCols / 8;
+  __shared__ __align__(16) uint32_t tile[kTRows][kTWords];
   const uint32_t ct = blockIdx.x % col_tiles;
   const int64_t row0 = (int64_t)(blockIdx.x / col_tiles) * kTRows;
-  const int col0 = ct * kTCols;
-  if constexpr (VEC) {
-    constexpr int kPer = 16 / sizeof(T), kChunks = kTCols / kPer;      // 16-byte chunks of a row
+  const uint32_t unit0 = ct * kUnitsPerRow;
+  constexpr int kStep = kMxThreads / kUnitsPerRow, kLoads = kTRows / kStep;   // a thread's units are kStep rows apart
+  const int c8 = threadIdx.x % kUnitsPerRow;
+  Raw8<D> raw[kLoads];
+  load_units<D, VEC>(x, row0 + threadIdx.x / kUnitsPerRow, kStep, (int)(unit0 + c8) * 8, cols, rows, raw);
 #pragma unroll
-    for (int i = threadIdx.x; i < kTRows * kChunks; i += kMxThreads) {
-      const int r = i / kChunks, c = (i % kChunks) * kPer;
-      const T* src = static_cast<const T*>(x.p) + (row0 + r) * x.ld + col0 + c;
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (row0 + r < rows) {
-        if (col0 + c + kPer <= cols) w = __ldg(reinterpret_cast<const uint4*>(src));
-        else {
-          T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-          for (int k = 0; k < kPer; ++k)
-            if (col0 + c + k < cols) e[k] = src[k];
-        }
-      }
-      *reinterpret_cast<uint4*>(&tile[r][c]) = w;
-    }
-  } else {
-    for (int i = threadIdx.x; i < kTRows * kTCols; i += kMxThreads) {
-      const int r = i / kTCols, c = i % kTCols;
-      tile[r][c] = row0 + r < rows && col0 + c < cols ? static_cast<const T*>(x.p)[(row0 + r) * x.ld + col0 + c] : (T)0;
+  for (int j = 0; j < kLoads; ++j) {
+    const int r = threadIdx.x / kUnitsPerRow + j * kStep, swap = ((r >> 5) & 3) << 3;
+    if constexpr (D == RT_F32) {
+      *reinterpret_cast<uint4*>(&tile[r][(c8 * 8) ^ swap]) = raw[j].w[0];
+      *reinterpret_cast<uint4*>(&tile[r][(c8 * 8 + 4) ^ swap]) = raw[j].w[1];
+    } else {
+      *reinterpret_cast<uint4*>(&tile[r][(c8 * 4) ^ swap]) = raw[j].w[0];
     }
   }
   __syncthreads();
-  const int c = threadIdx.x & (kTCols - 1), quarter = threadIdx.x / kTCols;
+  const int lane = threadIdx.x & 31, quarter = lane >> 3, wc = (threadIdx.x >> 5) * 8 + (lane & 7);
   const int nb = (int)((rows + 31) >> 5), b = (int)(row0 >> 5) + quarter;
-  const int out = col0 + c;
-  float v[4][8];
+  const uint32_t* column = &tile[quarter * 32][wc ^ (quarter << 3)];
   uint32_t amax = 0;
 #pragma unroll
-  for (int k = 0; k < 32; ++k) v[k >> 3][k & 7] = to_f32<D>(tile[quarter * 32 + k][c]);
+  for (int k = 0; k < 32; ++k) amax = amax_both<D>(amax, column[k * kTWords] & (D == RT_F32 ? 0x7FFFFFFFu : 0x7FFF7FFFu));
+  const int out0 = (int)ct * kTCols + wc * kPer;
+  uint32_t byte[kPer], q[kPer][4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) amax = max(amax, amax8(v[k]));
-  if (out < cols && b < nb) {
-    const uint32_t unit = (uint32_t)out * (nb * 4) + b * 4;
-    uint32_t byte, w[4];
+  for (int h = 0; h < kPer; ++h) byte[h] = byte_fp4(D == RT_F32 ? amax : amax_bits<D>(h ? amax & 0xFFFF0000u : amax & 0xFFFFu));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = codes_fp4<SR>(v[k], amax, byte, sr.keys, sr.tensor_id, sr.step, unit + k);
-    reinterpret_cast<uint4*>(codes)[(int64_t)out * nb + b] = make_uint4(w[0], w[1], w[2], w[3]);
-    put_fp4_scale(scales, nb, out, b, byte);
+  for (int k = 0; k < 4; ++k) {       // eight rows at a time, read again: 32 words would cost the registers of half the warps
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = column[(k * 8 + j) * kTWords];
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (D == RT_F32) v[j] = __uint_as_float(w[j]);
+        else v[j] = to_f32<D>((uint16_t)(h ? w[j] >> 16 : w[j] & 0xFFFFu));
+      }
+      q[h][k] = codes_fp4<SR>(v, byte[h], sr.keys, sr.tensor_id, sr.step, (uint32_t)(out0 + h) * (nb * 4) + b * 4 + k);
+    }
   }
+#pragma unroll
+  for (int h = 0; h < kPer; ++h)
+    if (out0 + h < cols && b < nb) {
+      reinterpret_cast<uint4*>(codes)[(int64_t)(out0 + h) * nb + b] = make_uint4(q[h][0], q[h][1], q[h][2], q[h][3]);
+      put_fp4_scale(scales + fp4_scale_at(out0 + h, b, (nb + 3) >> 2), nb, b, byte[h]);
+    }
   clear_fp4_pad(scales, cols, nb, blockIdx.x * kMxThreads + threadIdx.x, gridDim.x * kMxThreads);
 }
 
@@ -324,32 +420,26 @@ mx_quantize_t_kernel(const Matrix x, const int64_t rows, const int cols, const u
 template <int D, int FMT, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Grid g, const Matrix out) {
-  __shared__ float stage[VEC ? 1 : kMxWarps * 256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t first = blockIdx.x * (kMxThreads * kUnits) + threadIdx.x;
+  const Place<kRows> at(g);
   const int nb = g.upr.d >> 2;
-  uint2 w[kUnits];
-  uint32_t byte[kUnits];
+  uint2 w[kRows];
+  uint32_t byte[kRows];
+  const uint8_t* sp;
+  int stride;
+  if constexpr (FMT == RT_MXINT8) sp = int8_scale(const_cast<uint8_t*>(scales), g, at, stride);
+  else { sp = scales + fp4_scale_at(at.r, at.c8 >> 2, (nb + 3) >> 2); stride = 16; }
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    const uint32_t u = first + k * kMxThreads;
-    uint32_t r, c;
-    g.upr.split(u, r, c);
+  for (int k = 0; k < kRows; ++k) {
     w[k] = make_uint2(0u, 0u);
     byte[k] = 127;
-    if (u < g.units) {
-      if constexpr (FMT == RT_MXINT8) {
-        w[k] = __ldg(reinterpret_cast<const uint2*>(codes) + u);
-        byte[k] = __ldg(scales + (int64_t)r * ((nb + 3) & ~3) + (c >> 2));
-      } else {
-        w[k].x = __ldg(reinterpret_cast<const uint32_t*>(codes) + u);
-        byte[k] = __ldg(scales + fp4_scale_at(r, c >> 2, (nb + 3) >> 2));
-      }
+    if (at.live(g, k)) {
+      if constexpr (FMT == RT_MXINT8) w[k] = __ldg(reinterpret_cast<const uint2*>(codes) + at.unit(g, k));
+      else w[k].x = __ldg(reinterpret_cast<const uint32_t*>(codes) + at.unit(g, k));
+      byte[k] = __ldg(sp + k * stride);
     }
   }
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    const uint32_t u = first + k * kMxThreads;
+  for (int k = 0; k < kRows; ++k) {
     float x[8];
     if constexpr (FMT == RT_MXINT8) values_int8(w[k], scale_of(byte[k], 6), x);
     else values_fp4(w[k].x, scale_of(byte[k], 0), x);
@@ -357,41 +447,59 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = fabsf(x[j]) > 65504.f ? copysignf(65504.f, x[j]) : x[j];   // NaN stays
     }
-    if constexpr (VEC) {
-      uint32_t r, c;
-      g.upr.split(u, r, c);
-      if (u < g.units) store_unit<D>(out, g, r, c, x);
-    } else {
-      store_staged<D>(out, g, u - lane, lane, stage + warp * 256, x);
-    }
+    store_unit<D, VEC>(out, g.cols, at.r + k, at.c, at.live(g, k), x);
   }
 }
 
 // ------------------------------------------------------------------------------ gated activation
 // act(g) and act'(g).  For 16-bit results the exponential and the reciprocal are the hardware's
-// approximations (relative error about 2^-21 each, far below the 2^-9 of the result's rounding);
-// for fp32 results they are CUDA's functions.
+// approximations (relative error about 2^-22 each, far below the 2^-9 or 2^-12 of the result's
+// rounding), and the normal distribution comes of one exponential, which act' needs as well; for fp32
+// results they are CUDA's functions.
 template <bool EXACT>
-__device__ __forceinline__ float exp_of(float x) { return EXACT ? expf(x) : __expf(x); }
+__device__ __forceinline__ float exp_of(float x) {
+  if constexpr (EXACT) return expf(x);
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+  return y;
+}
 template <bool EXACT>
-__device__ __forceinline__ float sigmoid_of(float x) {
-  const float d = 1.f + exp_of<EXACT>(-x);
-  return EXACT ? 1.f / d : __fdividef(1.f, d);   // 2^126 < d < inf would make the quick division 0, and so it should
+__device__ __forceinline__ float reciprocal_of(float x) {
+  if constexpr (EXACT) return 1.f / x;
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 template <int ACT, bool EXACT>
 __device__ __forceinline__ void act_of(float g, float& a, float& d) {
   if constexpr (ACT == RT_ACT_SILU) {
-    const float s = sigmoid_of<EXACT>(g);
+    const float s = reciprocal_of<EXACT>(1.f + exp_of<EXACT>(-g));
     a = g * s;
-    d = s * (1.f + g * (1.f - s));
+    d = EXACT ? s * (1.f + g * (1.f - s)) : fmaf(a, 1.f - s, s);
   } else if constexpr (ACT == RT_ACT_GELU) {
-    const float p = 0.5f * erfcf(-0.70710678f * g);      // no cancellation for negative g
+    const float e = exp_of<EXACT>(-0.5f * g * g);
+    float p;
+    if constexpr (EXACT) {
+      p = 0.5f * erfcf(-0.70710678f * g);                // no cancellation for negative g
+    } else {
+      // exp(x^2) erfc(x) / t as a polynomial in t = 1 / (1 + 0.39 x), x = |g| / sqrt(2): fitted for the least relative
+      // error on x >= 0, 2.8e-6; times exp(-x^2) t / 2 that is the lower tail of the normal distribution
+      const float t = reciprocal_of<false>(fmaf(0.39f * 0.70710678f, fabsf(g), 1.f));
+      float q = fmaf(-0.10806743f, t, 0.2491668f);
+      q = fmaf(q, t, 0.018013082f);
+      q = fmaf(q, t, 0.20227431f);
+      q = fmaf(q, t, 0.19818425f);
+      q = fmaf(q, t, 0.22040357f);
+      q = fmaf(q, t, 0.22002489f);
+      const float tail = 0.5f * t * e * q;
+      p = g > 0.f ? 1.f - tail : tail;
+    }
     a = g * p;
-    d = p + 0.39894228f * g * exp_of<EXACT>(-0.5f * g * g);
+    d = fmaf(0.39894228f * g, e, p);
   } else {
     // beyond |g| = 16 the sigmoid is 0 or 1 and its slope 0; the cube must not reach infinity there (NaN passes)
     const float c = g > 16.f ? 16.f : g < -16.f ? -16.f : g, q = c * c;
-    const float s = sigmoid_of<EXACT>(1.59576912f * c * (1.f + 0.044715f * q));
+    const float s = reciprocal_of<EXACT>(1.f + exp_of<EXACT>(-1.59576912f * c * (1.f + 0.044715f * q)));
     a = g * s;
     d = s + c * s * (1.f - s) * 1.59576912f * (1.f + 0.134145f * q);
   }
@@ -402,85 +510,71 @@ struct Kept {              // an MXINT8 matrix
   uint8_t* scales;
 };
 
+constexpr int kPairs = 2;  // rows to a thread
+
 template <int D, int ACT, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, VEC && D != RT_F32 ? 5 : 1)
 mx_gated_kernel(const Matrix gate, const Matrix up, const Grid g, const Matrix h, const Kept kg, const Kept ku) {
-  __shared__ float stage_all[VEC ? 1 : kMxWarps * 256];
-  float* stage = stage_all + (VEC ? 0 : (threadIdx.x >> 5) * 256);
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = 2;
-  const uint32_t first = blockIdx.x * (kMxThreads * kPer) + threadIdx.x;
-  Raw8<D> ra[VEC ? kPer : 1], rb[VEC ? kPer : 1];
-  if constexpr (VEC) {
+  const Place<kPairs> at(g);
+  const int nb = g.upr.d >> 2;
+  Raw8<D> ra[kPairs], rb[kPairs];
+  load_units<D, VEC>(gate, at.r, 1, at.c, g.cols, g.rows, ra);
+  load_units<D, VEC>(up, at.r, 1, at.c, g.cols, g.rows, rb);
+  int stride;
+  uint8_t* sg = int8_scale(kg.scales, g, at, stride);
+  uint8_t* su = int8_scale(ku.scales, g, at, stride);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      const uint32_t u = first + k * kMxThreads;
-      uint32_t r, c;
-      g.upr.split(u, r, c);
-      ra[k] = load_unit<D>(gate, g, r, c, u < g.units);
-      rb[k] = load_unit<D>(up, g, r, c, u < g.units);
+  for (int k = 0; k < kPairs; ++k) {
+    const uint32_t ma = amax_of_block<D>(ra[k]), mb = amax_of_block<D>(rb[k]);
+    float a[8], b[8];
+    unpack<D>(ra[k], a);
+    unpack<D>(rb[k], b);
+    uint32_t ba, bb;
+    const uint2 wa = codes_int8(a, ma, ba), wb = codes_int8(b, mb, bb);
+    if (at.live(g, k)) {
+      const uint32_t u = at.unit(g, k);
+      reinterpret_cast<uint2*>(kg.codes)[u] = wa;
+      reinterpret_cast<uint2*>(ku.codes)[u] = wb;
+      put_int8_scale(sg + k * stride, nb, at.c8, ba);
+      put_int8_scale(su + k * stride, nb, at.c8, bb);
     }
-  }
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const uint32_t u = first + k * kMxThreads;
-    float a[8], b[8], y[8];
-    if constexpr (VEC) { unpack<D>(ra[k], a); unpack<D>(rb[k], b); }
-    else {
-      load_staged<D, VEC>(gate, g, u - lane, lane, stage, a);
-      load_staged<D, VEC>(up, g, u - lane, lane, stage, b);
-    }
-    const uint32_t ma = amax_of_four(amax8(a)), mb = amax_of_four(amax8(b));
-    uint32_t r, c, byte;
-    g.upr.split(u, r, c);
-    const uint2 wa = codes_int8(a, ma, byte);
-    if (u < g.units) put_int8(kg.codes, kg.scales, g, r, c, wa, byte);
-    const uint2 wb = codes_int8(b, mb, byte);
-    if (u < g.units) put_int8(ku.codes, ku.scales, g, r, c, wb, byte);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       float f, d;
       act_of<ACT, D == RT_F32>(a[j], f, d);
-      y[j] = f * b[j];
+      b[j] *= f;
     }
-    if constexpr (VEC) { if (u < g.units) store_unit<D>(h, g, r, c, y); }
-    else store_staged<D>(h, g, u - lane, lane, stage, y);
+    store_unit<D, VEC>(h, g.cols, at.r + k, at.c, at.live(g, k), b);
   }
 }
 
 template <int D, int ACT, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, VEC && D != RT_F32 ? 6 : 1)
 mx_gated_backward_kernel(const Matrix grad, const Kept kg, const Kept ku, const Grid g, const Matrix dgate, const Matrix dup) {
-  __shared__ float stage_all[VEC ? 1 : kMxWarps * 256];
-  float* stage = stage_all + (VEC ? 0 : (threadIdx.x >> 5) * 256);
-  const int lane = threadIdx.x & 31;
-  constexpr int kPer = 2;
-  const uint32_t first = blockIdx.x * (kMxThreads * kPer) + threadIdx.x;
-  const int stride = ((g.upr.d >> 2) + 3) & ~3;
-  Raw8<D> raw[VEC ? kPer : 1];
-  uint2 wg[kPer], wu[kPer];
-  uint32_t bg[kPer], bu[kPer];
+  const Place<kPairs> at(g);
+  Raw8<D> raw[kPairs];
+  uint2 wg[kPairs], wu[kPairs];
+  uint32_t bg[kPairs], bu[kPairs];
+  int stride;
+  const uint8_t* sg = int8_scale(kg.scales, g, at, stride);
+  const uint8_t* su = int8_scale(ku.scales, g, at, stride);
+  load_units<D, VEC>(grad, at.r, 1, at.c, g.cols, g.rows, raw);
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const uint32_t u = first + k * kMxThreads;
-    uint32_t r, c;
-    g.upr.split(u, r, c);
+  for (int k = 0; k < kPairs; ++k) {
     wg[k] = wu[k] = make_uint2(0u, 0u);
     bg[k] = bu[k] = 127u;
-    if (u < g.units) {
+    if (at.live(g, k)) {
+      const uint32_t u = at.unit(g, k);
       wg[k] = __ldg(reinterpret_cast<const uint2*>(kg.codes) + u);
       wu[k] = __ldg(reinterpret_cast<const uint2*>(ku.codes) + u);
-      bg[k] = __ldg(kg.scales + (int64_t)r * stride + (c >> 2));
-      bu[k] = __ldg(ku.scales + (int64_t)r * stride + (c >> 2));
+      bg[k] = __ldg(sg + k * stride);
+      bu[k] = __ldg(su + k * stride);
     }
-    if constexpr (VEC) raw[k] = load_unit<D>(grad, g, r, c, u < g.units);
   }
 #pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const uint32_t u = first + k * kMxThreads;
+  for (int k = 0; k < kPairs; ++k) {
     float dh[8], a[8], b[8];
-    if constexpr (VEC) unpack<D>(raw[k], dh);
-    else load_staged<D, VEC>(grad, g, u - lane, lane, stage, dh);
+    unpack<D>(raw[k], dh);
     values_int8(wg[k], scale_of(bg[k], 6), a);
     values_int8(wu[k], scale_of(bu[k], 6), b);
 #pragma unroll
@@ -490,17 +584,8 @@ mx_gated_backward_kernel(const Matrix grad, const Kept kg, const Kept ku, const 
       b[j] = dh[j] * b[j] * d;
       a[j] = dh[j] * f;
     }
-    if constexpr (VEC) {
-      uint32_t r, c;
-      g.upr.split(u, r, c);
-      if (u < g.units) {
-        store_unit<D>(dgate, g, r, c, b);
-        store_unit<D>(dup, g, r, c, a);
-      }
-    } else {
-      store_staged<D>(dgate, g, u - lane, lane, stage, b);
-      store_staged<D>(dup, g, u - lane, lane, stage, a);
-    }
+    store_unit<D, VEC>(dgate, g.cols, at.r + k, at.c, at.live(g, k), b);
+    store_unit<D, VEC>(dup, g.cols, at.r + k, at.c, at.live(g, k), a);
   }
 }
 
@@ -529,9 +614,11 @@ static int check_matrix(const void* p, int dtype, int64_t cols, int64_t ld, cons
 }
 static Grid grid_of(int64_t rows, int64_t cols) {
   const uint32_t upr = (uint32_t)(pad_to(cols, kMxBlock) / 8);
-  return {FastDiv::of(upr), (uint32_t)(rows * upr), (int)cols, (uint32_t)rows};
+  return {FastDiv::of(upr), (int)cols, (uint32_t)rows};
 }
-static unsigned blocks_for(uint32_t units, int per) { return (units + (uint32_t)per - 1) / (uint32_t)per; }
+static unsigned blocks_for(const Grid& g, int rows) {
+  return (unsigned)(((uint64_t)((g.rows + rows - 1) / rows) * g.upr.d + kMxThreads - 1) / kMxThreads);
+}
 static int launched() {
   stats().kernel_launches.fetch_add(1, std::memory_order_relaxed);
   RT_CUDA(cudaGetLastError());
@@ -542,6 +629,7 @@ template <int D>
 static void run_quantize(int fmt, bool transpose, bool sr, bool vec, const Matrix& x, int64_t rows, int64_t cols, uint8_t* codes,
                          uint8_t* scales, const SrArgs& args, cudaStream_t st) {
   if (transpose) {
+    constexpr int kTCols = kTWords * (D == RT_F32 ? 1 : 2);
     const uint32_t ct = (uint32_t)((cols + kTCols - 1) / kTCols);
     const unsigned nb = (unsigned)(ct * ((rows + kTRows - 1) / kTRows));
     auto k = sr ? (vec ? mx_quantize_t_kernel<D, true, true> : mx_quantize_t_kernel<D, true, false>)
@@ -553,25 +641,25 @@ static void run_quantize(int fmt, bool transpose, bool sr, bool vec, const Matri
   auto k = fmt == RT_MXINT8 ? (vec ? mx_quantize_kernel<D, RT_MXINT8, false, true> : mx_quantize_kernel<D, RT_MXINT8, false, false>)
            : sr             ? (vec ? mx_quantize_kernel<D, RT_MXFP4, true, true> : mx_quantize_kernel<D, RT_MXFP4, true, false>)
                             : (vec ? mx_quantize_kernel<D, RT_MXFP4, false, true> : mx_quantize_kernel<D, RT_MXFP4, false, false>);
-  k<<<blocks_for(g.units, kMxThreads * kUnits), kMxThreads, 0, st>>>(x, g, codes, scales, args);
+  k<<<blocks_for(g, kRows), kMxThreads, 0, st>>>(x, g, codes, scales, args);
 }
 
 template <int D>
 static void run_dequantize(int fmt, bool vec, const uint8_t* codes, const uint8_t* scales, const Grid& g, const Matrix& out, cudaStream_t st) {
   auto k = fmt == RT_MXINT8 ? (vec ? mx_dequantize_kernel<D, RT_MXINT8, true> : mx_dequantize_kernel<D, RT_MXINT8, false>)
                             : (vec ? mx_dequantize_kernel<D, RT_MXFP4, true> : mx_dequantize_kernel<D, RT_MXFP4, false>);
-  k<<<blocks_for(g.units, kMxThreads * kUnits), kMxThreads, 0, st>>>(codes, scales, g, out);
+  k<<<blocks_for(g, kRows), kMxThreads, 0, st>>>(codes, scales, g, out);
 }
 
 template <int D, int ACT>
 static void run_gated(bool vec, const Matrix& gate, const Matrix& up, const Grid& g, const Matrix& h, const Kept& kg, const Kept& ku, cudaStream_t st) {
   auto k = vec ? mx_gated_kernel<D, ACT, true> : mx_gated_kernel<D, ACT, false>;
-  k<<<blocks_for(g.units, kMxThreads * 2), kMxThreads, 0, st>>>(gate, up, g, h, kg, ku);
+  k<<<blocks_for(g, kPairs), kMxThreads, 0, st>>>(gate, up, g, h, kg, ku);
 }
 template <int D, int ACT>
 static void run_gated_backward(bool vec, const Matrix& grad, const Kept& kg, const Kept& ku, const Grid& g, const Matrix& dg, const Matrix& du, cudaStream_t st) {
   auto k = vec ? mx_gated_backward_kernel<D, ACT, true> : mx_gated_backward_kernel<D, ACT, false>;
-  k<<<blocks_for(g.units, kMxThreads * 2), kMxThreads, 0, st>>>(grad, kg, ku, g, dg, du);
+  k<<<blocks_for(g, kPairs), kMxThreads, 0, st>>>(grad, kg, ku, g, dg, du);
 }
 
 #define RT_BY_DTYPE(dtype, CALL)            \

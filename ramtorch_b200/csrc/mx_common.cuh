@@ -34,15 +34,11 @@ __device__ __forceinline__ float scale_of(uint32_t byte, int down) {
   return byte == 255u ? __uint_as_float(0x7FC00000u) : pow2f((int)byte - 127 - down);
 }
 
-// Block exponents from the bit pattern of the largest magnitude (finite): the smallest e with
-// amax <= 127 * 2^(e-6), and the smallest e with amax <= 6 * 2^e.
-__device__ __forceinline__ int exponent_int8(uint32_t amax) {
-  const int e = (int)(amax >> 23) - 127 + ((amax & 0x7FFFFFu) > 0x7E0000u);
-  return min(127, max(-120, e));
-}
-__device__ __forceinline__ int exponent_fp4(uint32_t amax) {
-  return max(-126, (int)(amax >> 23) - 129 + ((amax & 0x7FFFFFu) > 0x400000u));
-}
+// Scale bytes from the bit pattern of the largest magnitude (finite): e + 127 with the smallest e
+// such that amax <= 127 * 2^(e-6), and such that amax <= 6 * 2^e.  The addition carries into the exponent
+// exactly when the mantissa is above that of 127 / 64, and of 6 / 4.
+__device__ __forceinline__ uint32_t byte_of_int8(uint32_t amax) { return min(254u, max(7u, (amax + 0x1FFFFu) >> 23)); }
+__device__ __forceinline__ uint32_t byte_of_fp4(uint32_t amax) { return (uint32_t)max(1, (int)((amax + 0x3FFFFFu) >> 23) - 2); }
 
 // MXFP4 scales lie in tiles of 128 rows x 4 blocks (512 bytes), the order in which the tensor
 // core wants them: the 32 lanes of a tile row group, then its four groups, then the four blocks.

@@ -57,7 +57,8 @@ def quantize_fp4(x, draws=None):
         s = np.where(a < 2, 0.5, np.where(a < 4, 1.0, 2.0))
         v = np.floor(a / s + np.asarray(draws, np.float64).reshape(b.shape) / 65536) * s
         k = np.searchsorted(GRID, np.minimum(v, 6.0))
-    code = np.where(finite, k | (np.signbit(y) << 3), 0)
+    sign = np.signbit(y) if draws is None else np.signbit(y) & (k > 0)       # a zero that was drawn is +0
+    code = np.where(finite, k | (sign << 3), 0)
     v = np.where(finite, np.ldexp(np.where(np.signbit(y), -GRID[k], GRID[k]), e), np.nan)
     byte = np.where(finite, e + 127, 255)[..., 0]
     return code.reshape(len(b), -1).astype(np.uint8), byte.astype(np.uint8), v.reshape(len(b), -1)[:, :np.shape(x)[1]]
