@@ -78,17 +78,47 @@ __device__ __forceinline__ Raw8<D> load_unit(const elem_t<D>* p, const int c, co
   }
   return raw;
 }
-// the units of a thread; rows step rows apart
+// The units of a thread.  Where none of them needs a second look, which is nearly always, all loads
+// are issued before the first is used; a unit that may come in pieces would be waited for.
 template <int D, bool VEC, int R>
-__device__ __forceinline__ void load_units(const Matrix& m, int64_t row, int step, int c, int cols, int64_t rows, Raw8<D> (&raw)[R]) {
-  const elem_t<D>* p = static_cast<const elem_t<D>*>(m.p) + row * m.ld + c;
-  if (VEC && c + 8 <= cols && row + (R - 1) * step < rows) {      // nearly always: nothing to look at again
+__device__ __forceinline__ void load_units(const elem_t<D>* const (&p)[R], const int (&c)[R], const bool (&live)[R], const int cols, Raw8<D> (&raw)[R]) {
+  constexpr int kSize = sizeof(elem_t<D>), kWords = D == RT_F32 ? 2 : 1;
+  bool inner = true;
 #pragma unroll
-    for (int k = 0; k < R; ++k) raw[k] = load_raw<D>(p, k * step * m.ld);
+  for (int k = 0; k < R; ++k) inner = inner && live[k] && (VEC ? c[k] + 8 <= cols : c[k] >= 8 && c[k] + 8 + 16 / kSize <= cols);
+  if (inner) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) raw[k] = load_raw<D>(p[k], 0);
+    } else {
+      uint4 chunk[R][kWords + 1];
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int j = 0; j <= kWords; ++j) chunk[k][j] = __ldg(reinterpret_cast<const uint4*>((uintptr_t)p[k] & ~(uintptr_t)15) + j);
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) raw[k].w[j] = cut16(chunk[k][j], chunk[k][j + 1], (uint32_t)(uintptr_t)p[k] & 15u);
+    }
   } else {
 #pragma unroll
-    for (int k = 0; k < R; ++k) raw[k] = load_unit<D, VEC>(p + k * step * m.ld, c, cols, row + k * step < rows);
+    for (int k = 0; k < R; ++k) raw[k] = load_unit<D, VEC>(p[k], c[k], cols, live[k]);
   }
+}
+// of rows `step` apart
+template <int D, bool VEC, int R>
+__device__ __forceinline__ void load_rows(const Matrix& m, int64_t row, int step, int c, int cols, int64_t rows, Raw8<D> (&raw)[R]) {
+  const elem_t<D>* p[R];
+  int cs[R];
+  bool live[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    p[k] = static_cast<const elem_t<D>*>(m.p) + (row + k * step) * m.ld + c;
+    cs[k] = c;
+    live[k] = row + k * step < rows;
+  }
+  load_units<D, VEC, R>(p, cs, live, cols, raw);
 }
 template <int D>
 __device__ __forceinline__ void store_each(elem_t<D>* p, const float (&x)[8], int from, int to) {
@@ -262,7 +292,7 @@ __device__ __forceinline__ void values_int8(uint2 w, float s, float (&x)[8]) {
     const uint32_t u = (k < 2 ? w.x : w.y) ^ 0x80808080u;
     const float2 f = make_float2(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | ((2 * k) & 3))),
                                  __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 | ((2 * k + 1) & 3))));
-    const float2 v = mul2(add2_rz(f, make_float2(-8388736.f, -8388736.f)), make_float2(s, s));   // the sum is exact
+    const float2 v = mul2(make_float2(f.x - 8388736.f, f.y - 8388736.f), make_float2(s, s));
     x[2 * k] = v.x;
     x[2 * k + 1] = v.y;
   }
@@ -314,12 +344,12 @@ struct SrArgs {
 constexpr int kRows = 4;   // rows to a thread
 
 template <int D, int FMT, bool SR, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, SR || !VEC ? 1 : 6)
 mx_quantize_kernel(const Matrix x, const Grid g, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const SrArgs sr) {
   const Place<kRows> at(g);
   const int nb = g.upr.d >> 2;
   Raw8<D> raw[kRows];
-  load_units<D, VEC>(x, at.r, 1, at.c, g.cols, g.rows, raw);
+  load_rows<D, VEC>(x, at.r, 1, at.c, g.cols, g.rows, raw);
   int stride;
   uint8_t* sp;
   if constexpr (FMT == RT_MXINT8) sp = int8_scale(scales, g, at, stride);
@@ -368,16 +398,21 @@ mx_quantize_t_kernel(const Matrix x, const int64_t rows, const int cols, const u
   const uint32_t unit0 = ct * kUnitsPerRow;
   constexpr int kStep = kMxThreads / kUnitsPerRow, kLoads = kTRows / kStep;   // a thread's units are kStep rows apart
   const int c8 = threadIdx.x % kUnitsPerRow;
-  Raw8<D> raw[kLoads];
-  load_units<D, VEC>(x, row0 + threadIdx.x / kUnitsPerRow, kStep, (int)(unit0 + c8) * 8, cols, rows, raw);
+  constexpr int kBatch = VEC ? kLoads : kLoads / 2;      // two chunks to a unit: half as many at a time
 #pragma unroll
-  for (int j = 0; j < kLoads; ++j) {
-    const int r = threadIdx.x / kUnitsPerRow + j * kStep, swap = ((r >> 5) & 3) << 3;
-    if constexpr (D == RT_F32) {
-      *reinterpret_cast<uint4*>(&tile[r][(c8 * 8) ^ swap]) = raw[j].w[0];
-      *reinterpret_cast<uint4*>(&tile[r][(c8 * 8 + 4) ^ swap]) = raw[j].w[1];
-    } else {
-      *reinterpret_cast<uint4*>(&tile[r][(c8 * 4) ^ swap]) = raw[j].w[0];
+  for (int j0 = 0; j0 < kLoads; j0 += kBatch) {
+    Raw8<D> raw[kBatch];
+    const int r0 = threadIdx.x / kUnitsPerRow + j0 * kStep;
+    load_rows<D, VEC>(x, row0 + r0, kStep, (int)(unit0 + c8) * 8, cols, rows, raw);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int r = r0 + j * kStep, swap = ((r >> 5) & 3) << 3;
+      if constexpr (D == RT_F32) {
+        *reinterpret_cast<uint4*>(&tile[r][(c8 * 8) ^ swap]) = raw[j].w[0];
+        *reinterpret_cast<uint4*>(&tile[r][(c8 * 8 + 4) ^ swap]) = raw[j].w[1];
+      } else {
+        *reinterpret_cast<uint4*>(&tile[r][(c8 * 4) ^ swap]) = raw[j].w[0];
+      }
     }
   }
   __syncthreads();
@@ -518,8 +553,8 @@ mx_gated_kernel(const Matrix gate, const Matrix up, const Grid g, const Matrix h
   const Place<kPairs> at(g);
   const int nb = g.upr.d >> 2;
   Raw8<D> ra[kPairs], rb[kPairs];
-  load_units<D, VEC>(gate, at.r, 1, at.c, g.cols, g.rows, ra);
-  load_units<D, VEC>(up, at.r, 1, at.c, g.cols, g.rows, rb);
+  load_rows<D, VEC>(gate, at.r, 1, at.c, g.cols, g.rows, ra);
+  load_rows<D, VEC>(up, at.r, 1, at.c, g.cols, g.rows, rb);
   int stride;
   uint8_t* sg = int8_scale(kg.scales, g, at, stride);
   uint8_t* su = int8_scale(ku.scales, g, at, stride);
@@ -549,28 +584,33 @@ mx_gated_kernel(const Matrix gate, const Matrix up, const Grid g, const Matrix h
 }
 
 template <int D, int ACT, bool VEC>
-__global__ void __launch_bounds__(kMxThreads, VEC && D != RT_F32 ? 6 : 1)
+__global__ void __launch_bounds__(kMxThreads)
 mx_gated_backward_kernel(const Matrix grad, const Kept kg, const Kept ku, const Grid g, const Matrix dgate, const Matrix dup) {
-  const Place<kPairs> at(g);
+  const uint32_t first = blockIdx.x * (kMxThreads * kPairs) + threadIdx.x;   // here a thread's units are a CTA's width apart
+  const int stride = ((g.upr.d >> 2) + 3) & ~3;
   Raw8<D> raw[kPairs];
   uint2 wg[kPairs], wu[kPairs];
-  uint32_t bg[kPairs], bu[kPairs];
-  int stride;
-  const uint8_t* sg = int8_scale(kg.scales, g, at, stride);
-  const uint8_t* su = int8_scale(ku.scales, g, at, stride);
-  load_units<D, VEC>(grad, at.r, 1, at.c, g.cols, g.rows, raw);
+  uint32_t bg[kPairs], bu[kPairs], r[kPairs], c8[kPairs];
+  const elem_t<D>* p[kPairs];
+  int c[kPairs];
+  bool live[kPairs];
 #pragma unroll
   for (int k = 0; k < kPairs; ++k) {
+    const uint32_t u = first + k * kMxThreads;
+    g.upr.split(u, r[k], c8[k]);
+    c[k] = (int)c8[k] * 8;
+    live[k] = r[k] < g.rows;
+    p[k] = static_cast<const elem_t<D>*>(grad.p) + (int64_t)r[k] * grad.ld + c[k];
     wg[k] = wu[k] = make_uint2(0u, 0u);
     bg[k] = bu[k] = 127u;
-    if (at.live(g, k)) {
-      const uint32_t u = at.unit(g, k);
+    if (live[k]) {
       wg[k] = __ldg(reinterpret_cast<const uint2*>(kg.codes) + u);
       wu[k] = __ldg(reinterpret_cast<const uint2*>(ku.codes) + u);
-      bg[k] = __ldg(sg + k * stride);
-      bu[k] = __ldg(su + k * stride);
+      bg[k] = __ldg(kg.scales + (int64_t)r[k] * stride + (c8[k] >> 2));
+      bu[k] = __ldg(ku.scales + (int64_t)r[k] * stride + (c8[k] >> 2));
     }
   }
+  load_units<D, VEC, kPairs>(p, c, live, g.cols, raw);
 #pragma unroll
   for (int k = 0; k < kPairs; ++k) {
     float dh[8], a[8], b[8];
@@ -584,8 +624,8 @@ mx_gated_backward_kernel(const Matrix grad, const Kept kg, const Kept ku, const 
       b[j] = dh[j] * b[j] * d;
       a[j] = dh[j] * f;
     }
-    store_unit<D, VEC>(dgate, g.cols, at.r + k, at.c, at.live(g, k), b);
-    store_unit<D, VEC>(dup, g.cols, at.r + k, at.c, at.live(g, k), a);
+    store_unit<D, VEC>(dgate, g.cols, r[k], c[k], live[k], b);
+    store_unit<D, VEC>(dup, g.cols, r[k], c[k], live[k], a);
   }
 }
 
@@ -659,7 +699,7 @@ static void run_gated(bool vec, const Matrix& gate, const Matrix& up, const Grid
 template <int D, int ACT>
 static void run_gated_backward(bool vec, const Matrix& grad, const Kept& kg, const Kept& ku, const Grid& g, const Matrix& dg, const Matrix& du, cudaStream_t st) {
   auto k = vec ? mx_gated_backward_kernel<D, ACT, true> : mx_gated_backward_kernel<D, ACT, false>;
-  k<<<blocks_for(g, kPairs), kMxThreads, 0, st>>>(grad, kg, ku, g, dg, du);
+  k<<<(blocks_for(g, 1) + kPairs - 1) / kPairs, kMxThreads, 0, st>>>(grad, kg, ku, g, dg, du);
 }
 
 #define RT_BY_DTYPE(dtype, CALL)            \
