@@ -65,8 +65,9 @@ __device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col
 // The worker warps' part after the last product.  One CTA per tile: straight from tensor memory.
 // A cluster per tile (the sum is split over its CTAs): every CTA leaves its part in shared memory, then adds
 // up a share of the tile's columns over all of them, always in the order of their ranks.
+// `first`, `step`: the cluster's ranks that share this tile.
 template <int BN>
-__device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, int row0, int col0, int splits, float* parts, bool ok) {
+__device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, int row0, int col0, int splits, int first, int step, float* parts, bool ok) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
   const bool worker = warp >= kFirstWorker;
   if (worker) {
@@ -95,14 +96,14 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
     __syncwarp();
     cluster_sync();
     if (worker) {
-      const int rank = (int)cluster_rank(), i = threadIdx.x - kFirstWorker * 32;
+      const int rank = ((int)cluster_rank() - first) / step, i = threadIdx.x - kFirstWorker * 32;
       const int per = BN / splits;                                    // splits divides 8, BN is a multiple of 32
       const uint32_t base = smem_u32(parts);
       const int col = col0 + (i & 127);
       for (int c = rank * per + (i >> 7); c < (rank + 1) * per; c += 2) {
         if (row0 + c >= o.rows || col >= o.cols) continue;
         float v = 0.f;
-        for (int r = 0; r < splits; ++r) v += load_peer(base + (uint32_t)(c * 128 + (i & 127)) * 4, r);
+        for (int r = 0; r < splits; ++r) v += load_peer(base + (uint32_t)(c * 128 + (i & 127)) * 4, first + r * step);
         put_out(o, (int64_t)(row0 + c) * o.ld + col, v);
       }
     }
@@ -117,22 +118,28 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
 // ready for the tensor core; the codes' tile (8 KB) comes by TMA as bytes, the worker warps turn
 // it into bf16 (exact: a code times a power of two) in the swizzled layout.  fp32 and fp16
 // gradients arrive as up to three bf16 pieces that add up to them exactly; the pieces are further steps of the same sum.
+//
+// PAIR: two CTAs (ranks 2j and 2j + 1 of a cluster) make one product of 256 x BN, each with its own 128
+// features and half of the gradient's columns, so that the gradient's tile is fetched and read half as
+// often: one CTA's 40 KB a step at 128 x 256 keep the L2 busier than the tensor core (462 us of loads
+// alone at 8192 x 4096 x 11008).  Rank 2j issues the products; both CTAs' workers arrive at its barrier.
 constexpr int kTok = 64;
 
-template <int BN>
+template <int BN, bool PAIR>
 struct WgradSmem {
-  static constexpr int kCodes = 128 * kTok, kA = 128 * kTok * 2, kB = BN * kTok * 2;
-  static constexpr int kStage = kCodes + kA + kB;
-  static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 5 : 6;
+  static constexpr int kCols = PAIR ? BN / 2 : BN;                // gradient columns that this CTA fetches
+  static constexpr int kCodes = 128 * kTok, kA = 128 * kTok * 2, kB = kCols * kTok * 2, kScales = kTok * 4;
+  static constexpr int kStage = kCodes + kA + kB + kScales;
+  static constexpr int kStages = kCols == 256 ? 4 : kCols == 128 ? 5 : 6;
   static constexpr int kBytes = kStages * kStage + 1024 + 256;   // alignment, barriers
 };
 
 struct WgradArgs {
   const uint8_t* scales;
   int64_t ld_scales;
-  int tokens, blocks;                     // blocks of 32 along k
+  int tokens;
   int token_steps, pieces, splits;
-  int k_tiles, n_tiles;
+  int k_tiles, n_tiles;                   // k_tiles: of 256 features with PAIR, else of 128
   OutMatrix out;
 };
 
@@ -149,54 +156,58 @@ __device__ __forceinline__ __nv_bfloat162 bf16x2_scale(uint32_t byte) {
   return *reinterpret_cast<const __nv_bfloat162*>(&w);
 }
 
-template <int BN>
+template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
 mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_grad, const WgradArgs a) {
-  using S = WgradSmem<BN>;
+  using S = WgradSmem<BN, PAIR>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t tile_a = base, tile_b = tile_a + S::kStages * S::kA, codes = tile_b + S::kStages * S::kB;
-  const uint32_t bars = codes + S::kStages * S::kCodes;
+  const uint32_t scales = codes + S::kStages * S::kCodes, bars = scales + S::kStages * S::kScales;
   const uint32_t full = bars, empty = bars + 8 * S::kStages, conv = empty + 8 * S::kStages, done = conv + 8 * S::kStages, slot = done + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // tiles: groups of eight along n, k inside: the CTAs that run together share few tiles of either side
-  const int tile = blockIdx.x / a.splits, rank = blockIdx.x % a.splits;
+  constexpr int kCtas = PAIR ? 2 : 1;
+  const int in_cluster = blockIdx.x % (a.splits * kCtas), side = PAIR ? in_cluster & 1 : 0, split = in_cluster / kCtas;
+  const int tile = blockIdx.x / (a.splits * kCtas);
   const int per_group = 8 * a.k_tiles, group = tile / per_group, width = min(8, a.n_tiles - 8 * group);
   const int in_group = tile - group * per_group;
-  const int n0 = (group * 8 + in_group % width) * BN, k0 = (in_group / width) * 128;
+  const int n0 = (group * 8 + in_group % width) * BN, k0 = (in_group / width * kCtas + side) * 128;
   const int64_t steps = (int64_t)a.token_steps * a.pieces;
-  const int first = (int)(steps * rank / a.splits), last = (int)(steps * (rank + 1) / a.splits);
+  const int first = (int)(steps * split / a.splits), count = (int)(steps * (split + 1) / a.splits) - first;
+  const uint32_t leader = (uint32_t)(in_cluster & ~(kCtas - 1));
 
   if (warp == 0 && elect_one()) {
     prefetch_map(&map_codes);
     prefetch_map(&map_grad);
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(full + 8 * s, 1);
+      mbar_init(full + 8 * s, 1 + 32);       // the loads, and warp 3's lanes
       mbar_init(empty + 8 * s, 1);
-      mbar_init(conv + 8 * s, 8);
+      mbar_init(conv + 8 * s, 4 * kCtas);    // the four warps of a step, of both CTAs
     }
     mbar_init(done, 1);
     fence_barrier_init();
   }
   constexpr int kColumns = BN;
-  if (warp == 2) tmem_alloc(slot, kColumns);
+  if (warp == 2) tmem_alloc<PAIR>(slot, kColumns);
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();        // the other CTA's barriers are there
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
   bool ok = true;
 
   if (warp == 0) {
     if (elect_one()) {
       int piece = first / a.token_steps, t = first % a.token_steps, i = 0;
-      for (int it = first; it < last && ok; ++it, ++i) {
+      for (; i < count; ++i) {
         const int s = i % S::kStages;
         if (!(ok = mbar_wait(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
         mbar_expect(full + 8 * s, S::kCodes + S::kB);
         tma_load_2d(&map_codes, codes + s * S::kCodes, full + 8 * s, k0, t * kTok);
 #pragma unroll
-        for (int j = 0; j < BN / 64; ++j)
-          tma_load_3d(&map_grad, tile_b + s * S::kB + j * 8192, full + 8 * s, n0 + j * 64, t * kTok, piece);
+        for (int j = 0; j < S::kCols / 64; ++j)
+          tma_load_3d(&map_grad, tile_b + s * S::kB + j * 8192, full + 8 * s, n0 + side * S::kCols + j * 64, t * kTok, piece);
         if (++t == a.token_steps) { t = 0; ++piece; }
       }
       if (!ok)   // the loads in flight still write to this CTA's memory
@@ -206,70 +217,89 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
         }
     }
   } else if (warp == 1) {
-    if (elect_one()) {
-      constexpr uint32_t idesc = idesc_bf16_mn(128, BN);
-      for (int i = 0; i < last - first; ++i) {
+    if (side == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_bf16_mn(128 * kCtas, BN);
+      const uint16_t both = (uint16_t)(3u << leader);
+      for (int i = 0; i < count; ++i) {
         const int s = i % S::kStages, phase = (i / S::kStages) & 1;
         if (!(ok = mbar_wait(full + 8 * s, phase) && mbar_wait(conv + 8 * s, phase))) break;
         tc_fence_after();
         const uint64_t da = tile_desc(tile_a + s * S::kA, 8192, 1024), db = tile_desc(tile_b + s * S::kB, 8192, 1024);
 #pragma unroll
-        for (int kk = 0; kk < kTok / 16; ++kk) mma_bf16(tmem, da + kk * (2048 >> 4), db + kk * (2048 >> 4), idesc, i > 0 || kk > 0);
-        tc_commit(empty + 8 * s);
+        for (int kk = 0; kk < kTok / 16; ++kk) mma_bf16<PAIR>(tmem, da + kk * (2048 >> 4), db + kk * (2048 >> 4), idesc, i > 0 || kk > 0);
+        tc_commit<PAIR>(empty + 8 * s, both);
       }
-      tc_commit(done);
+      tc_commit<PAIR>(done, both);
     }
-  } else if (warp >= kFirstWorker) {
-    const int w = threadIdx.x - kFirstWorker * 32;
-    const int tok[2] = {w >> 3, (w + 256) >> 3}, f16 = w & 7;      // 16 codes each: token, sixteenth of the features
-    const int block = (k0 >> 5) + (f16 >> 1);
-    const uint8_t* sc = a.scales + block;
-    const bool has_block = block < a.blocks;
-    const uint32_t dst = (uint32_t)(f16 >> 2) * 8192, flip = (uint32_t)(f16 >> 2);   // the halves of a warp's lanes start with different chunks: no bank conflicts
+  } else if (warp == 3) {
+    // the scales of a step: one word (four blocks) to a token
+    const uint8_t* sc = a.scales + (k0 >> 5);
+    const bool some = (k0 >> 5) < a.ld_scales;      // the second CTA of the last pair may have nothing
     int t = first % a.token_steps;
-    uint32_t byte[2];
-    auto fetch = [&](int step) {
+    for (int i = 0; i < count; ++i) {
+      const int s = i % S::kStages;
+      if (!(ok = mbar_wait(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int token = step * kTok + tok[h];
-        byte[h] = has_block && token < a.tokens ? __ldg(sc + token * a.ld_scales) : 127u;
+        const int token = t * kTok + h * 32 + lane;
+        const bool live = some && token < a.tokens;
+        copy4(scales + s * S::kScales + (h * 32 + lane) * 4, live ? sc + token * a.ld_scales : a.scales, live);
       }
-    };
-    if (first < last) fetch(t);
-    for (int i = 0; i < last - first; ++i) {
-      const int s = i % S::kStages, phase = (i / S::kStages) & 1;
-      const __nv_bfloat162 scale[2] = {bf16x2_scale(byte[0]), bf16x2_scale(byte[1])};
+      copies_arrive(full + 8 * s);
       if (++t == a.token_steps) t = 0;
-      if (i + 1 < last - first) fetch(t);
-      if (!(ok = mbar_wait(full + 8 * s, phase))) break;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= kFirstWorker) {
+    // warps 4-7 take the even steps, 8-11 the odd ones; 64 codes to a thread
+    const int w = (threadIdx.x - kFirstWorker * 32) & 127, f16 = w & 7;                                    // sixteenth of the features
+    const uint32_t dst = (uint32_t)(f16 >> 2) * 8192, flip = (uint32_t)(f16 >> 2);   // the halves of a warp's lanes start with different chunks: no bank conflicts
+    const uint32_t c0 = (uint32_t)(f16 & 3) * 2, x = (uint32_t)(w >> 3) & 7u;      // the swizzle of tokens w/8, w/8 + 16, ... is the same
+    const uint32_t at0 = dst + (uint32_t)(w >> 3) * 128 + (((c0 + flip) ^ x) << 4), at1 = dst + (uint32_t)(w >> 3) * 128 + (((c0 + 1 - flip) ^ x) << 4);
+    const int mine = warp >= kFirstWorker + 4;
+    for (int i = 0; i < count; ++i) {
+      const int s = i % S::kStages, phase = (i / S::kStages) & 1;
+      if (!(ok = mbar_wait(full + 8 * s, phase))) break;      // every phase in turn: one that was left out could be taken for the next but one
+      if ((i & 1) != mine) continue;
+      const uint8_t* in = smem + (codes - base) + s * S::kCodes + (w >> 3) * 128 + f16 * 16;
+      const uint8_t* sc = smem + (scales - base) + s * S::kScales + (w >> 3) * 4 + (f16 >> 1);
+      uint8_t* out = smem + (tile_a - base) + s * S::kA;
+      uint4 c[4];
+      uint32_t byte[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 c = *reinterpret_cast<const uint4*>(smem + (codes - base) + s * S::kCodes + tok[h] * 128 + f16 * 16);
-        const uint32_t in[4] = {c.x, c.y, c.z, c.w};
+      for (int h = 0; h < 4; ++h) {
+        c[h] = *reinterpret_cast<const uint4*>(in + h * 16 * 128);
+        byte[h] = sc[h * 16 * 4];
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const __nv_bfloat162 scale = bf16x2_scale(byte[h]);
+        const uint32_t u[4] = {c[h].x, c[h].y, c[h].z, c[h].w};
         uint32_t v[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[2 * j] = bf16x2_of_codes(__byte_perm(in[j], 0u, 0x4140), scale[h]);
-          v[2 * j + 1] = bf16x2_of_codes(__byte_perm(in[j], 0u, 0x4342), scale[h]);
+          v[2 * j] = bf16x2_of_codes(__byte_perm(u[j], 0u, 0x4140), scale);
+          v[2 * j + 1] = bf16x2_of_codes(__byte_perm(u[j], 0u, 0x4342), scale);
         }
-        uint8_t* row = smem + (tile_a - base) + s * S::kA + dst + tok[h] * 128;
-        const uint32_t c0 = (uint32_t)(f16 & 3) * 2, x = (uint32_t)tok[h] & 7u;
         const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
-        *reinterpret_cast<uint4*>(row + (((c0 + flip) ^ x) << 4)) = flip ? hi : lo;
-        *reinterpret_cast<uint4*>(row + (((c0 + 1 - flip) ^ x) << 4)) = flip ? lo : hi;
+        *reinterpret_cast<uint4*>(out + at0 + h * 16 * 128) = flip ? hi : lo;
+        *reinterpret_cast<uint4*>(out + at1 + h * 16 * 128) = flip ? lo : hi;
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(conv + 8 * s);
+      if (lane == 0) {
+        if constexpr (PAIR) mbar_arrive_at(conv + 8 * s, leader);
+        else mbar_arrive(conv + 8 * s);
+      }
     }
     ok = mbar_wait(done, 0) && ok;
     tc_fence_after();
   }
   __syncwarp();
   if (!ok) atomicAdd(&g_wait_faults, 1u);
-  finish_tile<BN>(a.out, tmem, n0, k0, a.splits, reinterpret_cast<float*>(smem), ok);
+  finish_tile<BN>(a.out, tmem, n0, k0, a.splits, side, kCtas, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
-  if (warp == 2) tmem_free(tmem, kColumns);
+  if constexpr (PAIR) cluster_sync();        // the pair's products read both CTAs' memory, its barriers are in both
+  if (warp == 2) tmem_free<PAIR>(tmem, kColumns);
 }
 
 // A gradient that the tensor maps cannot take as it is (fp32, fp16, rows that do not start on 16-byte
@@ -354,7 +384,7 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
     mbar_init(done, 1);
     fence_barrier_init();
   }
-  if (warp == 2) tmem_alloc(slot, S::kColumns);
+  if (warp == 2) tmem_alloc<false>(slot, S::kColumns);
   __syncthreads();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
   bool ok = true;
@@ -396,9 +426,9 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         for (int kk = 0; kk < products; ++kk)
           mma_mxfp4(tmem, db + kk * 2, da + kk * 2, kk & 1 ? idesc_mxfp4(128, BN, 1) : idesc_mxfp4(128, BN, 0), sf + 4 * (kk >> 1),
                     sf + 8 + 4 * (kk >> 1), i > 0 || kk > 0);
-        tc_commit(empty + 8 * s);
+        tc_commit<false>(empty + 8 * s);
       }
-      tc_commit(done);
+      tc_commit<false>(done);
     }
   } else if (warp >= kFirstWorker) {
     ok = mbar_wait(done, 0);
@@ -406,9 +436,9 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
   }
   __syncwarp();
   if (!ok) atomicAdd(&g_wait_faults, 1u);
-  finish_tile<BN>(a.out, tmem, m0, n0, a.splits, reinterpret_cast<float*>(smem), ok);
+  finish_tile<BN>(a.out, tmem, m0, n0, a.splits, 0, 1, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
-  if (warp == 2) tmem_free(tmem, S::kColumns);
+  if (warp == 2) tmem_free<false>(tmem, S::kColumns);
 }
 
 static int check_out(const void* out, int dtype, int64_t cols, int64_t ld) {
@@ -449,10 +479,10 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, i
   return 0;
 }
 
-// Launch a tensor-core kernel as clusters of `splits` CTAs.  Its shared memory is raised once per
+// Launch a tensor-core kernel as clusters of `cluster` CTAs.  Its shared memory is raised once per
 // device and kernel.
 template <typename K, typename... Args>
-static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t ctas, int splits, cudaStream_t st, Args... args) {
+static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t ctas, int cluster, cudaStream_t st, Args... args) {
   int device = 0;
   RT_CUDA(cudaGetDevice(&device));
   if (device >= 64 || !(raised.load(std::memory_order_acquire) >> device & 1)) {
@@ -466,19 +496,20 @@ static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t 
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)splits;
+  at.val.clusterDim.x = (unsigned)cluster;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
   RT_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
   stats().kernel_launches.fetch_add(1, std::memory_order_relaxed);
   return 0;
 }
 
-template <int BN>
+template <int BN, bool PAIR>
 static int run_wgrad(const CUtensorMap& codes, const CUtensorMap& grad, const WgradArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
-  return launch_tc(mx_weight_grad_kernel<BN>, raised, WgradSmem<BN>::kBytes, (int64_t)a.k_tiles * a.n_tiles * a.splits, a.splits, st, codes, grad, a);
+  const int cluster = a.splits * (PAIR ? 2 : 1);
+  return launch_tc(mx_weight_grad_kernel<BN, PAIR>, raised, WgradSmem<BN, PAIR>::kBytes, (int64_t)a.k_tiles * a.n_tiles * cluster, cluster, st, codes, grad, a);
 }
 
 template <int BN>
@@ -530,31 +561,29 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   const int pieces = need ? pieces_of(grad_dtype) : 1;
   WgradArgs a{};
   a.scales = (const uint8_t*)scales;
-  a.blocks = (int)(kp / kMxBlock);
-  a.ld_scales = pad_to(a.blocks, 4);
+  a.ld_scales = pad_to(kp / kMxBlock, 4);
   a.tokens = (int)tokens;
   a.token_steps = (int)((tokens + kTok - 1) / kTok);
   a.pieces = pieces;
   a.out = {out, ld_out, (int)n, (int)k, out_dtype, accumulate != 0};
 
-  // Tile width and split.  A step costs what the longer of the product and the conversion costs;
-  // a CTA also pays for its start, its output and, when split, the exchange (clocks, measured).
+  // Tile and split.  A step costs what the longest of product, conversion and loads costs; a CTA
+  // also pays for its start, its output and, when split, the exchange (clocks, measured).
   const int64_t steps = (int64_t)a.token_steps * pieces;
-  const int64_t k_tiles = (k + 127) / 128;
-  int bn = 256, splits = 1;
+  struct Shape { int bn, ctas; double step; };
+  static const Shape shapes[] = {{256, 2, 620}, {128, 1, 500}, {64, 1, 400}};
+  const Shape* pick = nullptr;
   double best = 1e300;
-  for (const int width : {256, 128, 64})
-    for (const int s : {1, 2, 4, 8}) {
+  for (const Shape& c : shapes)
+    for (int s = 1; s * c.ctas <= 8; s *= 2) {
       if (s > steps) continue;
-      const double step = width == 256 ? 700 : width == 128 ? 400 : 300;
-      const int64_t ctas = k_tiles * ((n + width - 1) / width) * s;
-      const double cost = (double)((ctas + kSms - 1) / kSms) * ((double)((steps + s - 1) / s) * step + 3000 + width * 12 + (s > 1 ? 2500 : 0));
-      if (cost < best) { best = cost; bn = width; splits = s; }
+      const int64_t ctas = (k + 128 * c.ctas - 1) / (128 * c.ctas) * c.ctas * ((n + c.bn - 1) / c.bn) * s;
+      const double cost = (double)((ctas + kSms - 1) / kSms) * ((double)((steps + s - 1) / s) * c.step + 3000 + c.bn * 12 + (s > 1 ? 2500 : 0));
+      if (cost < best) { best = cost; pick = &c; a.splits = s; }
     }
-  a.splits = splits;
-  a.k_tiles = (int)k_tiles;
-  a.n_tiles = (int)((n + bn - 1) / bn);
-  if (k_tiles * a.n_tiles * splits > 0x7FFFFFFFll) return fail(RT_E_SIZE, "n * k is too large");
+  a.k_tiles = (int)((k + 128 * pick->ctas - 1) / (128 * pick->ctas));
+  a.n_tiles = (int)((n + pick->bn - 1) / pick->bn);
+  if ((int64_t)a.k_tiles * a.n_tiles * a.splits * pick->ctas > 0x7FFFFFFFll) return fail(RT_E_SIZE, "n * k is too large");
 
   CUtensorMap map_codes, map_grad;
   {
@@ -575,9 +604,9 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
     else spread_gradient_kernel<RT_BF16, 1><<<nb, 256, 0, st>>>((const uint16_t*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
     if (int rc = launched()) return rc;
   }
-  if (bn == 256) return run_wgrad<256>(map_codes, map_grad, a, st);
-  if (bn == 128) return run_wgrad<128>(map_codes, map_grad, a, st);
-  return run_wgrad<64>(map_codes, map_grad, a, st);
+  if (pick->bn == 256) return run_wgrad<256, true>(map_codes, map_grad, a, st);
+  if (pick->bn == 128) return run_wgrad<128, false>(map_codes, map_grad, a, st);
+  return run_wgrad<64, false>(map_codes, map_grad, a, st);
 }
 
 extern "C" int rt_mx_wait_faults(uint32_t* count) {

@@ -35,18 +35,20 @@ __device__ __forceinline__ uint64_t nanoseconds() {
 // No wait of a correct launch comes near that: the bound is there so that a mistake ends the
 // kernel instead of hanging the GPU.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity) {
+__device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity) {
   const uint64_t began = nanoseconds();
   do {
 #pragma unroll 1
-    for (int i = 0; i < 256; ++i)
+    for (int i = 0; i < 1024; ++i)
       if (mbar_try(bar, parity)) return true;
   } while (nanoseconds() - began < kWaitLimitNs);
   return false;
 }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-  if (mbar_try(bar, parity)) return true;
-  return mbar_wait_slow(bar, parity);
+#pragma unroll 1
+  for (int i = 0; i < 4096; ++i)            // reading the clock takes longer than most waits
+    if (mbar_try(bar, parity)) return true;
+  return mbar_wait_long(bar, parity);
 }
 
 __device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
@@ -76,19 +78,39 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "r"(bar) : "memory");
 }
 
-// --------------------------------------------------------------------------------- tensor memory
-__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {   // one whole warp
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// four bytes, zeros where `live` is false; and an arrival at `bar` when this thread's copies so far are done
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4u : 0u) : "memory");
 }
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// --------------------------------------------------------------------------------- tensor memory
+// One whole warp; with PAIR one warp of each of the two CTAs.  A kernel uses either form throughout.
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+}
+template <bool PAIR>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// arrives at `bar` when all products issued so far by this thread are done
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// arrives at `bar` when all products issued so far by this thread are done; with PAIR at both CTAs' barriers of that place
+template <bool PAIR>
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint16_t ctas = 0) {
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(ctas) : "memory");
+  else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 32 consecutive columns of this warp's quarter of the lanes: register j of lane l is (lane l, column j)
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
@@ -123,10 +145,16 @@ __device__ __forceinline__ uint64_t plain_desc(uint32_t addr, uint32_t lead, uin
 __host__ __device__ constexpr uint32_t idesc_bf16_mn(int m, int n) {
   return 1u << 4 | 1u << 7 | 1u << 10 | 1u << 15 | 1u << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
 }
 
 // MXFP4 x MXFP4 -> fp32, 64 columns of the sum: two blocks, whose scales are bytes 2 * half and 2 * half + 1 of a word of tensor memory
@@ -152,6 +180,12 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrives at the barrier that CTA `rank` of the cluster has at the place of `bar`.  A release at cluster
+// scope would wait for all of this thread's memory traffic (0.3 us); what the arrival announces are
+// writes to this CTA's own shared memory, which fence_proxy_async has completed.
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+  asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tmbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar), "r"(rank) : "memory");
 }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
   float v;

@@ -600,3 +600,32 @@ def test_no_wait_ran_out():
     torch.cuda.synchronize()
     count = ctypes.c_uint32(99)
     assert N.lib().rt_mx_wait_faults(ctypes.byref(count)) == 0 and count.value == 0
+
+
+@gpu
+@pytest.mark.parametrize("tokens,n,k", [(64, 256, 256), (100, 300, 130), (700, 2100, 2500), (2000, 500, 4096), (320, 4000, 4500)])
+def test_weight_gradient_of_many_tiles(tokens, n, k):
+    """Enough tiles, or tokens, for every tile shape and split; the last tiles of both sides are cut."""
+    x = U.matrix(tokens, k, "bf16", 15, 1.0, DEV)
+    g = U.matrix(tokens, n, "bf16", 16, 1e-2, DEV, loud=False)
+    q = mx.quantize_mxint8(x)
+    xv, gv = q.dequantize(torch.float32).double(), g.double()
+    exact, mags = np64(gv.T @ xv), np64(gv.T.abs() @ xv.abs())
+    buf, out = guarded(n, k, "f32", k + 9)
+    mx.weight_grad(g, q, out=out)
+    assert (np.abs(np64(out) - exact) <= sum_bound("f32", tokens, exact, mags)).all()
+    assert untouched(buf, n, k)
+    assert (np.abs(np64(mx.weight_grad(g, q)) - exact) <= sum_bound("bf16", tokens, exact, mags)).all()
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(129, 300, 700), (700, 2100, 512), (2000, 500, 1024), (320, 4000, 300), (1, 20000, 4096), (60, 5000, 2080)])
+def test_fp4_product_of_many_tiles(m, n, k):
+    a = mx.quantize_mxfp4(U.matrix(m, k, "bf16", 17, 1.0, DEV))
+    b = mx.quantize_mxfp4(U.matrix(n, k, "bf16", 18, 0.02, DEV))
+    av, bv = a.dequantize(torch.float32).double(), b.dequantize(torch.float32).double()
+    exact, mags = np64(av @ bv.T), np64(av.abs() @ bv.abs().T)
+    buf, out = guarded(m, n, "f32", n + 9)
+    mx.mxfp4_matmul(a, b, out=out)
+    assert (np.abs(np64(out) - exact) <= sum_bound("f32", k, exact, mags)).all()
+    assert untouched(buf, m, n)
