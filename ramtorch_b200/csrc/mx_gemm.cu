@@ -132,6 +132,7 @@ struct WgradSmem {
   static constexpr int kStage = kCodes + kA + kB + kScales;
   static constexpr int kStages = kCols == 256 ? 4 : kCols == 128 ? 5 : 6;
   static constexpr int kBytes = kStages * kStage + 1024 + 256;   // alignment, barriers
+  static constexpr int kN = BN > 256 ? 256 : BN;                  // columns to a product; BN / kN products share A
 };
 
 struct WgradArgs {
@@ -143,17 +144,21 @@ struct WgradArgs {
   OutMatrix out;
 };
 
-// two codes in the low bytes of the halves of a word -> two bf16 integers: with the byte c = low7 - (sign bit),
-// 128 + low7 and 128 + (sign bit) are bf16 numbers made by setting bits, their difference is exact
-__device__ __forceinline__ uint32_t bf16x2_of_codes(uint32_t w, __nv_bfloat162 scale) {
-  const uint32_t x = (w & 0x007F007Fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y)), scale);
+// Two codes in the low bytes of the halves of a word -> two bf16 numbers code * 2^(byte - 133).  With
+// code = low7 - 128 * (top bit), (128 + low7) * 2^m and (128 + 128 * (top bit)) * 2^m are bf16 numbers made by
+// setting and adding bits to k = the bits of 128 * 2^m, m = byte - 133, and their difference is exact.  k is
+// (byte + 1) << 7, which has an exponent for every byte up to 252; a warp that meets a larger one
+// (values from 2^119 on, or NaN) multiplies by the scale instead.
+__device__ __forceinline__ uint32_t bf16x2_of_codes(uint32_t w, uint32_t k) {
+  const uint32_t x = (w & 0x007F007Fu) | k, y = (w & 0x00800080u) + k;
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ __nv_bfloat162 bf16x2_scale(uint32_t byte) {
-  const uint32_t h = byte == 255u ? 0x7FC0u : byte >= 7u ? (byte - 6u) << 7 : 1u << byte;   // 2^(byte - 133)
-  const uint32_t w = h | h << 16;
-  return *reinterpret_cast<const __nv_bfloat162*>(&w);
+constexpr uint32_t kByteOfOne = 133;     // the scale byte of 2^0
+__device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t byte) {
+  const uint32_t h = byte == 255u ? 0x7FC0u : byte >= 7u ? (byte - 6u) << 7 : 1u << byte, w = h | h << 16;   // 2^(byte - 133)
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&w));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 template <int BN, bool PAIR>
@@ -190,7 +195,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     mbar_init(done, 1);
     fence_barrier_init();
   }
-  constexpr int kColumns = BN;
+  constexpr int kColumns = BN, kHalfN = S::kN / kCtas;     // columns of one product that this CTA holds
   if (warp == 2) tmem_alloc<PAIR>(slot, kColumns);
   __syncthreads();
   if constexpr (PAIR) cluster_sync();        // the other CTA's barriers are there
@@ -207,7 +212,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
         tma_load_2d(&map_codes, codes + s * S::kCodes, full + 8 * s, k0, t * kTok);
 #pragma unroll
         for (int j = 0; j < S::kCols / 64; ++j)
-          tma_load_3d(&map_grad, tile_b + s * S::kB + j * 8192, full + 8 * s, n0 + side * S::kCols + j * 64, t * kTok, piece);
+          tma_load_3d(&map_grad, tile_b + s * S::kB + j * 8192, full + 8 * s, n0 + (j * 64 / kHalfN) * S::kN + side * kHalfN + j * 64 % kHalfN, t * kTok, piece);
         if (++t == a.token_steps) { t = 0; ++piece; }
       }
       if (!ok)   // the loads in flight still write to this CTA's memory
@@ -218,7 +223,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     }
   } else if (warp == 1) {
     if (side == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_bf16_mn(128 * kCtas, BN);
+      constexpr uint32_t idesc = idesc_bf16_mn(128 * kCtas, S::kN);
       const uint16_t both = (uint16_t)(3u << leader);
       for (int i = 0; i < count; ++i) {
         const int s = i % S::kStages, phase = (i / S::kStages) & 1;
@@ -226,7 +231,10 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
         tc_fence_after();
         const uint64_t da = tile_desc(tile_a + s * S::kA, 8192, 1024), db = tile_desc(tile_b + s * S::kB, 8192, 1024);
 #pragma unroll
-        for (int kk = 0; kk < kTok / 16; ++kk) mma_bf16<PAIR>(tmem, da + kk * (2048 >> 4), db + kk * (2048 >> 4), idesc, i > 0 || kk > 0);
+        for (int kk = 0; kk < kTok / 16; ++kk)
+#pragma unroll
+          for (int j = 0; j < BN / S::kN; ++j)
+            mma_bf16<PAIR>(tmem + j * S::kN, da + kk * (2048 >> 4), db + ((j * kHalfN * kTok * 2 + kk * 2048) >> 4), idesc, i > 0 || kk > 0);
         tc_commit<PAIR>(empty + 8 * s, both);
       }
       tc_commit<PAIR>(done, both);
@@ -250,39 +258,45 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= kFirstWorker) {
-    // warps 4-7 take the even steps, 8-11 the odd ones; 64 codes to a thread
-    const int w = (threadIdx.x - kFirstWorker * 32) & 127, f16 = w & 7;                                    // sixteenth of the features
-    const uint32_t dst = (uint32_t)(f16 >> 2) * 8192, flip = (uint32_t)(f16 >> 2);   // the halves of a warp's lanes start with different chunks: no bank conflicts
-    const uint32_t c0 = (uint32_t)(f16 & 3) * 2, x = (uint32_t)(w >> 3) & 7u;      // the swizzle of tokens w/8, w/8 + 16, ... is the same
-    const uint32_t at0 = dst + (uint32_t)(w >> 3) * 128 + (((c0 + flip) ^ x) << 4), at1 = dst + (uint32_t)(w >> 3) * 128 + (((c0 + 1 - flip) ^ x) << 4);
+    // Warps 4-7 take the even steps, 8-11 the odd ones; 64 codes to a thread, 16 of them (a chunk of the
+    // codes, two of the bf16 tile) at a time.  Lanes 0-3 and 4-7, and so on, have tokens that differ in bits 0 and 2: with
+    // both tiles' chunks exchanged by the token's low bits (128-byte swizzle), eight lanes then read eight
+    // different chunks of a row and write eight different ones.
+    const int w = warp & 3, sub = lane & 3, pair = lane >> 3, low = lane & 4 ? pair ^ 5 : pair;      // low: token & 7
     const int mine = warp >= kFirstWorker + 4;
     for (int i = 0; i < count; ++i) {
       const int s = i % S::kStages, phase = (i / S::kStages) & 1;
       if (!(ok = mbar_wait(full + 8 * s, phase))) break;      // every phase in turn: one that was left out could be taken for the next but one
       if ((i & 1) != mine) continue;
-      const uint8_t* in = smem + (codes - base) + s * S::kCodes + (w >> 3) * 128 + f16 * 16;
-      const uint8_t* sc = smem + (scales - base) + s * S::kScales + (w >> 3) * 4 + (f16 >> 1);
-      uint8_t* out = smem + (tile_a - base) + s * S::kA;
+      const uint8_t* in = smem + (codes - base) + s * S::kCodes + (w * 16 + low) * 128;
+      const uint8_t* sc = smem + (scales - base) + s * S::kScales + (w * 16 + low) * 4;
+      uint8_t* out = smem + (tile_a - base) + s * S::kA + (w * 16 + low) * 128;
       uint4 c[4];
       uint32_t byte[4];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        c[h] = *reinterpret_cast<const uint4*>(in + h * 16 * 128);
-        byte[h] = sc[h * 16 * 4];
+      for (int h = 0; h < 4; ++h) {      // token groups h / 2, feature halves h % 2
+        c[h] = *reinterpret_cast<const uint4*>(in + (h >> 1) * 1024 + ((((h & 1) * 4 + sub) ^ low) << 4));
+        byte[h] = sc[(h >> 1) * 32 + (h & 1) * 2 + (sub >> 1)];
       }
+      const bool large = max(max(byte[0], byte[1]), max(byte[2], byte[3])) > 252u;
+      const bool slow = __any_sync(0xFFFFFFFFu, large);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const __nv_bfloat162 scale = bf16x2_scale(byte[h]);
+        const uint32_t k = ((slow ? kByteOfOne : byte[h]) + 1u) * 0x00800080u;
         const uint32_t u[4] = {c[h].x, c[h].y, c[h].z, c[h].w};
         uint32_t v[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          v[2 * j] = bf16x2_of_codes(__byte_perm(u[j], 0u, 0x4140), scale);
-          v[2 * j + 1] = bf16x2_of_codes(__byte_perm(u[j], 0u, 0x4342), scale);
+          v[2 * j] = bf16x2_of_codes(__byte_perm(u[j], 0u, 0x4140), k);
+          v[2 * j + 1] = bf16x2_of_codes(__byte_perm(u[j], 0u, 0x4342), k);
         }
-        const uint4 lo = make_uint4(v[0], v[1], v[2], v[3]), hi = make_uint4(v[4], v[5], v[6], v[7]);
-        *reinterpret_cast<uint4*>(out + at0 + h * 16 * 128) = flip ? hi : lo;
-        *reinterpret_cast<uint4*>(out + at1 + h * 16 * 128) = flip ? lo : hi;
+        if (slow) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = scaled(v[j], byte[h]);
+        }
+        uint8_t* row = out + (h >> 1) * 1024 + (h & 1) * 8192;
+        *reinterpret_cast<uint4*>(row + (((sub * 2) ^ low) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<uint4*>(row + (((sub * 2 + 1) ^ low) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
       }
       fence_proxy_async();
       __syncwarp();
@@ -571,12 +585,12 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   // also pays for its start, its output and, when split, the exchange (clocks, measured).
   const int64_t steps = (int64_t)a.token_steps * pieces;
   struct Shape { int bn, ctas; double step; };
-  static const Shape shapes[] = {{256, 2, 620}, {128, 1, 500}, {64, 1, 400}};
+  static const Shape shapes[] = {{512, 2, 1100}, {256, 2, 650}, {128, 1, 500}, {64, 1, 400}};
   const Shape* pick = nullptr;
   double best = 1e300;
   for (const Shape& c : shapes)
     for (int s = 1; s * c.ctas <= 8; s *= 2) {
-      if (s > steps) continue;
+      if (s > steps || (s > 1 && c.bn > 256)) continue;      // a split tile has to fit into shared memory
       const int64_t ctas = (k + 128 * c.ctas - 1) / (128 * c.ctas) * c.ctas * ((n + c.bn - 1) / c.bn) * s;
       const double cost = (double)((ctas + kSms - 1) / kSms) * ((double)((steps + s - 1) / s) * c.step + 3000 + c.bn * 12 + (s > 1 ? 2500 : 0));
       if (cost < best) { best = cost; pick = &c; a.splits = s; }
@@ -589,7 +603,7 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   {
     const uint64_t dims[2] = {(uint64_t)kp, (uint64_t)tokens}, strides[1] = {(uint64_t)kp};
     const uint32_t box[2] = {128, (uint32_t)kTok};
-    if (int rc = make_map(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    if (int rc = make_map(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   }
   {
     const int64_t ld = need ? np : ld_grad;
@@ -604,6 +618,7 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
     else spread_gradient_kernel<RT_BF16, 1><<<nb, 256, 0, st>>>((const uint16_t*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
     if (int rc = launched()) return rc;
   }
+  if (pick->bn == 512) return run_wgrad<512, true>(map_codes, map_grad, a, st);
   if (pick->bn == 256) return run_wgrad<256, true>(map_codes, map_grad, a, st);
   if (pick->bn == 128) return run_wgrad<128, false>(map_codes, map_grad, a, st);
   return run_wgrad<64, false>(map_codes, map_grad, a, st);
