@@ -73,37 +73,55 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return OUT
 
 
-FASTSCAN_SRC = os.path.join(HERE, "fastscan.cpp")
-FASTSCAN_OUT = os.path.join(PKG, "_fastscan.so")
-
-
-def build_fastscan(force: bool = False) -> str:
-    """Build ``ramtorch_b200/_fastscan.so``, the host-side helper that walks long parameter lists in
-    C++ (g++ against the torch headers of the running interpreter).  It only reads tensor pointers
-    and properties; the optimizer works without it, with per-tensor Python passes instead."""
-    if not force and os.path.exists(FASTSCAN_OUT) and os.path.getmtime(FASTSCAN_OUT) >= os.path.getmtime(FASTSCAN_SRC):
-        return FASTSCAN_OUT
+def _build_module(name: str, src: str, out: str, force: bool, deps=(), cuda: bool = False) -> str:
+    """Build an optional host-side helper with g++ against the torch headers of the running interpreter."""
+    if not force and os.path.exists(out) and all(os.path.getmtime(out) >= os.path.getmtime(d) for d in (src, *deps)):
+        return out
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension as ce
     gxx = shutil.which("g++")
     if not gxx:
-        raise RuntimeError("g++ not found: _fastscan.so cannot be built")
+        raise RuntimeError(f"g++ not found: {name}.so cannot be built")
     inc = ce.include_paths() + [sysconfig.get_paths()["include"]]
     libs = ce.library_paths()
     cmd = [gxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-DTORCH_EXTENSION_NAME=_fastscan", "-DTORCH_API_INCLUDE_EXTENSION_H"]
-    cmd += [f"-I{i}" for i in inc] + [FASTSCAN_SRC, "-o", FASTSCAN_OUT + ".tmp"]
-    cmd += [f"-L{d}" for d in libs] + [f"-Wl,-rpath,{d}" for d in libs] + ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+           f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H"]
+    link = ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10"]
+    if cuda:
+        inc.append(os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"))
+        link += ["-ltorch_cuda", "-lc10_cuda"]
+    cmd += [f"-I{i}" for i in inc] + [src, "-o", out + ".tmp"]
+    cmd += [f"-L{d}" for d in libs] + [f"-Wl,-rpath,{d}" for d in libs] + link
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("g++ failed building _fastscan.so")
-    os.replace(FASTSCAN_OUT + ".tmp", FASTSCAN_OUT)
-    return FASTSCAN_OUT
+        raise RuntimeError(f"g++ failed building {name}.so")
+    os.replace(out + ".tmp", out)
+    return out
+
+
+FASTSCAN_SRC = os.path.join(HERE, "fastscan.cpp")
+FASTSCAN_OUT = os.path.join(PKG, "_fastscan.so")
+MXCALL_SRC = os.path.join(HERE, "mxcall.cpp")
+MXCALL_OUT = os.path.join(PKG, "_mxcall.so")
+
+
+def build_fastscan(force: bool = False) -> str:
+    """Build ``ramtorch_b200/_fastscan.so``, the host-side helper that walks long parameter lists in
+    C++.  It only reads tensor pointers and properties; the optimizer works without it, with
+    per-tensor Python passes instead."""
+    return _build_module("_fastscan", FASTSCAN_SRC, FASTSCAN_OUT, force)
+
+
+def build_mxcall(force: bool = False) -> str:
+    """Build ``ramtorch_b200/_mxcall.so``, the host side of the microscaled calls in C++ (allocation, current device
+    and stream, the call of the C ABI).  ``microscaling`` works without it, through ctypes."""
+    return _build_module("_mxcall", MXCALL_SRC, MXCALL_OUT, force, deps=(os.path.join(ROOT, "include", "rt_b200.h"),), cuda=True)
 
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
     print(build_fastscan(force="--force" in sys.argv))
+    print(build_mxcall(force="--force" in sys.argv))

@@ -30,6 +30,26 @@ _FORMATS = {"mxint8": N.MXINT8, "mxfp4": N.MXFP4}
 _CODES_DTYPE = {"mxint8": torch.int8, "mxfp4": torch.uint8}
 
 
+_fast = None        # the C++ host side: a module, or False where it is not built
+
+
+def _helper():
+    """``_mxcall.so`` with the library's entry points handed to it, or ``False``."""
+    global _fast
+    if _fast is None:
+        try:
+            from . import _mxcall
+        except ImportError:
+            _fast = False
+        else:
+            L = N.lib()
+            _mxcall.init({name: ctypes.cast(getattr(L, name), ctypes.c_void_p).value
+                          for name in ("rt_last_error", "rt_mx_quantize", "rt_mx_dequantize", "rt_mx_gated_act", "rt_mx_gated_act_backward",
+                                       "rt_mx_weight_grad_workspace", "rt_mx_weight_grad", "rt_mxfp4_matmul")})
+            _fast = _mxcall
+    return _fast
+
+
 def _pad(n: int, to: int) -> int:
     return (n + to - 1) // to * to
 
@@ -77,13 +97,17 @@ class MxTensor:
         self.format, self.codes, self.scales, self.shape, self.dtype = format, codes, scales, shape, dtype
 
     @classmethod
-    def _new(cls, fmt, shape, rows, cols, dtype, device):
+    def _of(cls, fmt, codes, scales, shape, dtype):
+        """From arrays that this module laid out itself."""
         t = object.__new__(cls)
-        codes, scales = _layout(fmt, rows, cols)
-        t.format, t.shape, t.dtype = fmt, shape, dtype
-        t.codes = torch.empty(codes, dtype=_CODES_DTYPE[fmt], device=device)
-        t.scales = torch.empty(scales, dtype=torch.uint8, device=device)
+        t.format, t.codes, t.scales, t.shape, t.dtype = fmt, codes, scales, shape, dtype
         return t
+
+    @classmethod
+    def _new(cls, fmt, shape, rows, cols, dtype, device):
+        codes, scales = _layout(fmt, rows, cols)
+        return cls._of(fmt, torch.empty(codes, dtype=_CODES_DTYPE[fmt], device=device),
+                       torch.empty(scales, dtype=torch.uint8, device=device), shape, dtype)
 
     @property
     def device(self) -> torch.device:
@@ -108,6 +132,9 @@ class MxTensor:
             dtype = dtype or self.dtype
             if dtype not in N.DTYPE_CODE:
                 raise ValueError(f"unsupported dtype {dtype} (bf16, fp32, fp16 only)")
+            fast = _fast or _helper()
+            if fast:
+                return fast.dequantize(_FORMATS[self.format], self.codes, self.scales, rows, cols, self.shape, N.DTYPE_CODE[dtype])
             out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
             ld = cols
         else:
@@ -183,33 +210,29 @@ def _same_place(t, device, name):
         raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
-def _draws(seed, tensor_id, step):
-    if seed is None:
-        return None
-    if not (0 <= tensor_id < 2**32 and 0 <= step < 2**32):
-        raise ValueError("tensor_id and step must fit 32 bits")
-    return N.MxDraws(seed & (2**64 - 1), tensor_id, step)
-
-
-def _quantize(x, fmt, transpose, draws):
+def _quantize(x, fmt, transpose, seed, tensor_id, step):
     rows, cols, ld = _rows(x, "x")
-    if transpose:
-        if x.dim() != 2:
-            raise ValueError("transpose needs a matrix")
-        q = MxTensor._new(fmt, (cols, rows), cols, rows, x.dtype, x.device)
-    else:
-        q = MxTensor._new(fmt, tuple(x.shape), rows, cols, x.dtype, x.device)
+    if transpose and x.dim() != 2:
+        raise ValueError("transpose needs a matrix")
+    shape = (cols, rows) if transpose else tuple(x.shape)
+    if seed is not None and not (0 <= tensor_id < 2**32 and 0 <= step < 2**32):
+        raise ValueError("tensor_id and step must fit 32 bits")
+    fast = _fast or _helper()
+    if fast:
+        codes, scales = fast.quantize(x, rows, cols, ld, _FORMATS[fmt], transpose, seed is not None, (seed or 0) & (2**64 - 1), tensor_id, step)
+        return MxTensor._of(fmt, codes, scales, shape, x.dtype)
+    q = MxTensor._new(fmt, shape, cols if transpose else rows, rows if transpose else cols, x.dtype, x.device)
+    draws = None if seed is None else ctypes.byref(N.MxDraws(seed & (2**64 - 1), tensor_id, step))
     with _on(x.device):
         N.check(N.lib().rt_mx_quantize(x.data_ptr(), N.DTYPE_CODE[x.dtype], rows, cols, ld, _FORMATS[fmt], transpose,
-                                       q.codes.data_ptr(), q.scales.data_ptr(), None if draws is None else ctypes.byref(draws),
-                                       N.stream_ptr(x.device.index)), "rt_mx_quantize")
+                                       q.codes.data_ptr(), q.scales.data_ptr(), draws, N.stream_ptr(x.device.index)), "rt_mx_quantize")
     return q
 
 
 def quantize_mxint8(x: torch.Tensor) -> MxTensor:
     """``x`` (bf16, fp32 or fp16; leading dimensions count as rows, rows may be strided) in MXINT8, rounded
     to nearest: at most half of 2^-6 of the block's scale off."""
-    return _quantize(x, "mxint8", False, None)
+    return _quantize(x, "mxint8", False, None, 0, 0)
 
 
 def quantize_mxfp4(x: torch.Tensor, *, transpose: bool = False, seed: int | None = None, tensor_id: int = 0,
@@ -217,7 +240,7 @@ def quantize_mxfp4(x: torch.Tensor, *, transpose: bool = False, seed: int | None
     """``x`` in MXFP4, rounded to nearest, or with ``seed`` stochastically with the Philox draws
     ``(seed, tensor_id, step)``: unbiased, the same bits on every run.  ``transpose=True`` quantises
     ``x.T`` of a matrix, in blocks along x's rows, without forming it."""
-    return _quantize(x, "mxfp4", bool(transpose), _draws(seed, tensor_id, step))
+    return _quantize(x, "mxfp4", bool(transpose), seed, tensor_id, step)
 
 
 def mxfp4_matmul(a: MxTensor, b: MxTensor, *, dtype=None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -234,7 +257,11 @@ def mxfp4_matmul(a: MxTensor, b: MxTensor, *, dtype=None, out: torch.Tensor | No
     _same_place(b, a.device, "b")
     shape = a.shape[:-1] + (n,)
     if out is None:
-        out = torch.empty(shape, dtype=_out_dtype(dtype or a.dtype), device=a.device)
+        dtype = _out_dtype(dtype or a.dtype)
+        fast = _fast or _helper()
+        if fast:
+            return fast.matmul(a.codes, a.scales, b.codes, b.scales, m, n, k, shape, N.DTYPE_CODE[dtype])
+        out = torch.empty(shape, dtype=dtype, device=a.device)
         ld = n
     else:
         ld = _check_out(out, shape, dtype, a.device)
@@ -275,10 +302,15 @@ def weight_grad(grad_out: torch.Tensor, x8: MxTensor, *, dtype=None, out: torch.
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty((n, k), dtype=_out_dtype(dtype or grad_out.dtype), device=grad_out.device)
-        ld_out = k
+        dtype, ld_out = _out_dtype(dtype or grad_out.dtype), k
     else:
         ld_out = _check_out(out, (n, k), dtype, grad_out.device)
+        dtype = out.dtype
+    fast = _fast or _helper()
+    if fast:
+        return fast.weight_grad(grad_out, ld, x8.codes, x8.scales, tokens, n, k, out, ld_out, N.DTYPE_CODE[dtype], accumulate)
+    if out is None:
+        out = torch.empty((n, k), dtype=dtype, device=grad_out.device)
     L, code, g = N.lib(), N.DTYPE_CODE[grad_out.dtype], grad_out.data_ptr()
     need = L.rt_mx_weight_grad_workspace(g, code, ld, tokens, n, k)
     if need < 0:
@@ -309,6 +341,10 @@ def gated_act(gate: torch.Tensor, up: torch.Tensor, act: str = "silu"):
         raise ValueError("gate and up differ in shape or dtype")
     _same_place(up, gate.device, "up")
     shape, device = tuple(gate.shape), gate.device
+    fast = _fast or _helper()
+    if fast:
+        h, gc, gs, uc, us = fast.gated_act(gate, ld_gate, up, ld_up, rows, cols, code)
+        return h, MxTensor._of("mxint8", gc, gs, shape, gate.dtype), MxTensor._of("mxint8", uc, us, shape, gate.dtype)
     h = torch.empty(shape, dtype=gate.dtype, device=device)
     g8 = MxTensor._new("mxint8", shape, rows, cols, gate.dtype, device)
     u8 = MxTensor._new("mxint8", shape, rows, cols, gate.dtype, device)
@@ -330,6 +366,9 @@ def gated_act_backward(grad_h: torch.Tensor, gate8: MxTensor, up8: MxTensor, act
         if t.shape != tuple(grad_h.shape):
             raise ValueError(f"grad_h and {name} differ in shape")
         _same_place(t, grad_h.device, name)
+    fast = out is None and (_fast or _helper())
+    if fast:
+        return fast.gated_act_backward(grad_h, ld, rows, cols, code, gate8.codes, gate8.scales, up8.codes, up8.scales)
     if out is None:
         dgate, dup = torch.empty_like(grad_h, memory_format=torch.contiguous_format), torch.empty_like(grad_h, memory_format=torch.contiguous_format)
         ld_gate = ld_up = cols

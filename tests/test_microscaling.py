@@ -629,3 +629,29 @@ def test_fp4_product_of_many_tiles(m, n, k):
     mx.mxfp4_matmul(a, b, out=out)
     assert (np.abs(np64(out) - exact) <= sum_bound("f32", k, exact, mags)).all()
     assert untouched(buf, m, n)
+
+
+@gpu
+def test_both_host_sides_give_the_same(monkeypatch):
+    """With the C++ host side and through ctypes: the same results and the same refusals."""
+    x = torch.randn(3, 50, 264, device=DEV).bfloat16()
+    g = torch.randn(3, 50, 72, device=DEV).bfloat16()
+    w = torch.randn(72, 264, device=DEV).bfloat16()
+
+    def everything():
+        q, p = mx.quantize_mxint8(x), mx.quantize_mxfp4(x, seed=2**40 + 3, tensor_id=5, step=6)
+        t = mx.quantize_mxfp4(w, transpose=True)
+        h, g8, u8 = mx.gated_act(x[..., :130], x[..., 132:262])
+        out = torch.ones(72, 264, device=DEV)
+        found = [q.codes, q.scales, p.codes, p.scales, t.codes, t.scales, q.dequantize(), p.dequantize(torch.float32), t.dequantize(torch.float16),
+                 h, g8.codes, u8.scales, *mx.gated_act_backward(h, g8, u8), mx.weight_grad(g, q), mx.weight_grad(g.float(), q),
+                 mx.weight_grad(g, q, out=out, accumulate=True), mx.mxfp4_matmul(p, mx.quantize_mxfp4(w)), mx.mxfp4_matmul(p, mx.quantize_mxfp4(w), dtype=torch.float32)]
+        assert p.shape == (3, 50, 264) and t.shape == (264, 72) and found[-1].shape == (3, 50, 72) and found[9].shape == (3, 50, 130)
+        with pytest.raises(ValueError):
+            mx.quantize_mxint8(torch.empty(0, device=DEV).as_strided((0, 1 << 31), (1, 1)))
+        return found
+
+    a = everything()
+    monkeypatch.setattr(mx, "_fast", False)
+    for s, t in zip(a, everything()):
+        assert s.dtype == t.dtype and torch.equal(s, t)
