@@ -22,14 +22,17 @@ int mx_check_codes(const void* codes, const void* scales);
 __device__ unsigned int g_wait_faults;   // waits that ran out; see rt_mx_wait_faults
 
 constexpr int kSms = 148;
-constexpr int kTcThreads = 384;          // warp 0: loads, 1: products, 2: tensor memory, 4-11: conversion and output
-constexpr int kFirstWorker = 4;
+constexpr int kFirstWorker = 4;          // warp 0: loads, 1: products, 2: tensor memory, 3: scales, from 4: conversion and output
+constexpr int kConvGroups = 2;           // of four warps each, in the weight gradient's kernel
+constexpr int kWgradThreads = 32 * (kFirstWorker + 4 * kConvGroups);
+constexpr int kFp4Threads = 32 * (kFirstWorker + 8);
 
 struct OutMatrix {
   void* p;
   int64_t ld;
   int rows, cols;                        // the accumulator's columns / lanes
   int dtype, accumulate;
+  int wide;                              // rows start on 16-byte boundaries
 };
 
 template <int D>
@@ -42,51 +45,101 @@ __device__ __forceinline__ void put_out(const OutMatrix& o, int64_t at, float v)
   else if (o.dtype == RT_F32) put_one<RT_F32>(o, at, v);
   else put_one<RT_F16>(o, at, v);
 }
-// 32 columns of the accumulator that this warp holds, to 32 output rows
+// 16 columns of the accumulator that this warp holds, to 16 output rows
 template <int D>
-__device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col, const uint32_t (&acc)[32]) {
+__device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col, const uint32_t (&acc)[16]) {
   if (col >= o.cols) return;
   elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + (int64_t)row * o.ld + col;
-  const int live = min(32, o.rows - row);
+  const int live = min(16, o.rows - row);
   if (o.accumulate) {
-    float old[32];
+    float old[16];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) old[j] = j < live ? to_f32<D>(p[j * o.ld]) : 0.f;
+    for (int j = 0; j < 16; ++j) old[j] = j < live ? to_f32<D>(p[j * o.ld]) : 0.f;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < 16; ++j)
       if (j < live) p[j * o.ld] = of_f32<D>(old[j] + __uint_as_float(acc[j]));
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < 16; ++j)
       if (j < live) p[j * o.ld] = of_f32<D>(__uint_as_float(acc[j]));
   }
+}
+
+// 32 columns of the accumulator, from this warp's quarter of the lanes, as 32 output rows of 32 values:
+// through 32 x 32 values of shared memory that the warp has to itself, so that a lane stores 16 bytes
+// of one row.  Straight from the registers, 64 bytes of one row to a warp, a column of a tile took 17 ns, this
+// way 8; TMA stores from shared memory were no faster.
+template <int D>
+__device__ __forceinline__ void put_square(const OutMatrix& o, uint32_t tmem, int row, int col, elem_t<D>* room) {
+  constexpr int kLanes = D == RT_F32 ? 8 : 4, kPer = 32 / kLanes;     // lanes to a row, values to a lane
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t acc[16];
+    tmem_load16(tmem + 16 * h, acc);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if constexpr (D == RT_F32) room[(16 * h + j) * 32 + lane] = __uint_as_float(acc[j]);
+      else room[(16 * h + j) * 32 + lane] = of_f32<D>(__uint_as_float(acc[j]));
+    }
+  }
+  __syncwarp();
+  const int c = col + lane % kLanes * kPer;
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i) {
+    const int r = i * kPer + lane / kLanes;
+    if (row + r < o.rows && c < o.cols) {
+      const uint4 v = *reinterpret_cast<const uint4*>(room + r * 32 + lane % kLanes * kPer);
+      elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + (int64_t)(row + r) * o.ld + c;
+      if (c + kPer <= o.cols) *reinterpret_cast<uint4*>(p) = v;
+      else {
+        const elem_t<D>* e = reinterpret_cast<const elem_t<D>*>(&v);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k)
+          if (c + k < o.cols) p[k] = e[k];
+      }
+    }
+  }
+  __syncwarp();
 }
 
 // The worker warps' part after the last product.  One CTA per tile: straight from tensor memory.
 // A cluster per tile (the sum is split over its CTAs): every CTA leaves its part in shared memory, then adds
 // up a share of the tile's columns over all of them, always in the order of their ranks.
 // `first`, `step`: the cluster's ranks that share this tile.
-template <int BN>
+template <int BN, int WORKERS>
 __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, int row0, int col0, int splits, int first, int step, float* parts, bool ok) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
   const bool worker = warp >= kFirstWorker;
   if (worker) {
-    constexpr int kHalf = BN >= 64 ? BN / 2 : BN;
-    const int c0 = (warp - kFirstWorker) >= 4 ? kHalf : 0;
-    if (c0 < BN && ok) {
+    constexpr int kGroups = WORKERS / 4;
+    const int group = (warp - kFirstWorker) / 4;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+    if (ok) {
 #pragma unroll 1
-      for (int c = c0; c < c0 + kHalf; c += 32) {
-        uint32_t acc[32];
-        tmem_load32(tmem + ((uint32_t)(q * 32) << 16) + c, acc);
+      for (int c = group * 32; c < BN; c += kGroups * 32) {       // the groups of four warps take 32 columns in turn
         if (splits == 1) {
-          if (row0 + c < o.rows) {
-            if (o.dtype == RT_BF16) put_columns<RT_BF16>(o, row0 + c, col0 + q * 32 + lane, acc);
-            else if (o.dtype == RT_F32) put_columns<RT_F32>(o, row0 + c, col0 + q * 32 + lane, acc);
-            else put_columns<RT_F16>(o, row0 + c, col0 + q * 32 + lane, acc);
+          if (row0 + c >= o.rows) break;
+          if (o.wide && !o.accumulate) {
+            float* room = parts + (warp - kFirstWorker) * 1024;
+            if (o.dtype == RT_BF16) put_square<RT_BF16>(o, lanes + c, row0 + c, col0 + q * 32, reinterpret_cast<uint16_t*>(room));
+            else if (o.dtype == RT_F32) put_square<RT_F32>(o, lanes + c, row0 + c, col0 + q * 32, room);
+            else put_square<RT_F16>(o, lanes + c, row0 + c, col0 + q * 32, reinterpret_cast<uint16_t*>(room));
+            continue;
           }
-        } else {
+        }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) parts[(c + j) * 128 + q * 32 + lane] = __uint_as_float(acc[j]);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t acc[16];
+          tmem_load16(lanes + c + 16 * h, acc);
+          if (splits == 1) {
+            if (o.dtype == RT_BF16) put_columns<RT_BF16>(o, row0 + c + 16 * h, col0 + q * 32 + lane, acc);
+            else if (o.dtype == RT_F32) put_columns<RT_F32>(o, row0 + c + 16 * h, col0 + q * 32 + lane, acc);
+            else put_columns<RT_F16>(o, row0 + c + 16 * h, col0 + q * 32 + lane, acc);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) parts[(c + 16 * h + j) * 128 + q * 32 + lane] = __uint_as_float(acc[j]);
+          }
         }
       }
     }
@@ -96,15 +149,23 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
     __syncwarp();
     cluster_sync();
     if (worker) {
-      const int rank = ((int)cluster_rank() - first) / step, i = threadIdx.x - kFirstWorker * 32;
-      const int per = BN / splits;                                    // splits divides 8, BN is a multiple of 32
+      const int rank = ((int)cluster_rank() - first) / step;
       const uint32_t base = smem_u32(parts);
-      const int col = col0 + (i & 127);
-      for (int c = rank * per + (i >> 7); c < (rank + 1) * per; c += 2) {
-        if (row0 + c >= o.rows || col >= o.cols) continue;
-        float v = 0.f;
-        for (int r = 0; r < splits; ++r) v += load_peer(base + (uint32_t)(c * 128 + (i & 127)) * 4, first + r * step);
-        put_out(o, (int64_t)(row0 + c) * o.ld + col, v);
+      for (int e = threadIdx.x - kFirstWorker * 32; e < (BN + splits - 1) / splits * 32; e += WORKERS * 32) {   // four lanes of one column
+        const int c = rank + (e >> 5) * splits, f = (e & 31) * 4, col = col0 + f;
+        if (c >= BN) break;
+        float4 v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (r < splits) v[r] = load_peer(base + (uint32_t)(c * 128 + f) * 4, first + r * step);
+        float sum[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+        for (int r = 1; r < 8; ++r)
+          if (r < splits) { sum[0] += v[r].x; sum[1] += v[r].y; sum[2] += v[r].z; sum[3] += v[r].w; }
+        if (row0 + c < o.rows)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col + j < o.cols) put_out(o, (int64_t)(row0 + c) * o.ld + col + j, sum[j]);
       }
     }
     __syncwarp();
@@ -162,9 +223,10 @@ __device__ __forceinline__ uint32_t scaled(uint32_t v, uint32_t byte) {
 }
 
 template <int BN, bool PAIR>
-__global__ void __launch_bounds__(kTcThreads, 1)
+__global__ void __launch_bounds__(kWgradThreads, 1)
 mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __grid_constant__ CUtensorMap map_grad, const WgradArgs a) {
   using S = WgradSmem<BN, PAIR>;
+  static_assert(BN > 256 || BN * 512 <= S::kStages * S::kStage, "a part of a split tile");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
@@ -258,16 +320,16 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= kFirstWorker) {
-    // Warps 4-7 take the even steps, 8-11 the odd ones; 64 codes to a thread, 16 of them (a chunk of the
+    // Two groups of four warps take the steps in turn (four groups were no faster); 64 codes to a thread, 16 of them (a chunk of the
     // codes, two of the bf16 tile) at a time.  Lanes 0-3 and 4-7, and so on, have tokens that differ in bits 0 and 2: with
     // both tiles' chunks exchanged by the token's low bits (128-byte swizzle), eight lanes then read eight
     // different chunks of a row and write eight different ones.
     const int w = warp & 3, sub = lane & 3, pair = lane >> 3, low = lane & 4 ? pair ^ 5 : pair;      // low: token & 7
-    const int mine = warp >= kFirstWorker + 4;
+    const int mine = (warp - kFirstWorker) >> 2;
     for (int i = 0; i < count; ++i) {
       const int s = i % S::kStages, phase = (i / S::kStages) & 1;
       if (!(ok = mbar_wait(full + 8 * s, phase))) break;      // every phase in turn: one that was left out could be taken for the next but one
-      if ((i & 1) != mine) continue;
+      if (i % kConvGroups != mine) continue;
       const uint8_t* in = smem + (codes - base) + s * S::kCodes + (w * 16 + low) * 128;
       const uint8_t* sc = smem + (scales - base) + s * S::kScales + (w * 16 + low) * 4;
       uint8_t* out = smem + (tile_a - base) + s * S::kA + (w * 16 + low) * 128;
@@ -278,8 +340,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
         c[h] = *reinterpret_cast<const uint4*>(in + (h >> 1) * 1024 + ((((h & 1) * 4 + sub) ^ low) << 4));
         byte[h] = sc[(h >> 1) * 32 + (h & 1) * 2 + (sub >> 1)];
       }
-      const bool large = max(max(byte[0], byte[1]), max(byte[2], byte[3])) > 252u;
-      const bool slow = __any_sync(0xFFFFFFFFu, large);
+      const bool slow = __any_sync(0xFFFFFFFFu, max(max(byte[0], byte[1]), max(byte[2], byte[3])) > 252u);
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const uint32_t k = ((slow ? kByteOfOne : byte[h]) + 1u) * 0x00800080u;
@@ -310,7 +371,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
   }
   __syncwarp();
   if (!ok) atomicAdd(&g_wait_faults, 1u);
-  finish_tile<BN>(a.out, tmem, n0, k0, a.splits, side, kCtas, reinterpret_cast<float*>(smem), ok);
+  finish_tile<BN, 4 * kConvGroups>(a.out, tmem, n0, k0, a.splits, side, kCtas, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
   if constexpr (PAIR) cluster_sync();        // the pair's products read both CTAs' memory, its barriers are in both
   if (warp == 2) tmem_free<PAIR>(tmem, kColumns);
@@ -371,9 +432,10 @@ struct Fp4Args {
 };
 
 template <int BN>
-__global__ void __launch_bounds__(kTcThreads, 2)
+__global__ void __launch_bounds__(kFp4Threads, 2)
 mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp4Args a) {
   using S = Fp4Smem<BN>;
+  static_assert(BN * 512 <= S::kStages * S::kStage, "a part of a split tile");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
@@ -450,7 +512,7 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
   }
   __syncwarp();
   if (!ok) atomicAdd(&g_wait_faults, 1u);
-  finish_tile<BN>(a.out, tmem, m0, n0, a.splits, 0, 1, reinterpret_cast<float*>(smem), ok);
+  finish_tile<BN, 8>(a.out, tmem, m0, n0, a.splits, 0, 1, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
   if (warp == 2) tmem_free<false>(tmem, S::kColumns);
 }
@@ -496,7 +558,7 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, i
 // Launch a tensor-core kernel as clusters of `cluster` CTAs.  Its shared memory is raised once per
 // device and kernel.
 template <typename K, typename... Args>
-static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t ctas, int cluster, cudaStream_t st, Args... args) {
+static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int threads, int smem, int64_t ctas, int cluster, cudaStream_t st, Args... args) {
   int device = 0;
   RT_CUDA(cudaGetDevice(&device));
   if (device >= 64 || !(raised.load(std::memory_order_acquire) >> device & 1)) {
@@ -505,7 +567,7 @@ static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t 
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kTcThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute at{};
@@ -519,17 +581,51 @@ static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int smem, int64_t 
   return 0;
 }
 
+// How many clusters of `cluster` CTAs of a kernel the device runs at once: fewer than its SMs would
+// hold, since a cluster stays within a group of SMs (15 of eight CTAs, 33 of four on 148 SMs).  Asked once
+// per device, kernel and size.
+template <typename K>
+static int clusters_at_once(K kernel, std::atomic<int> (&known)[64][9], int threads, int smem, int cluster) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) { cudaGetLastError(); return kSms / cluster; }
+  std::atomic<int>* slot = device < 64 ? &known[device][cluster] : nullptr;
+  int n = slot ? slot->load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)cluster * 1024);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)cluster;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    return std::max(1, kSms / cluster);
+  }
+  if (slot) slot->store(n, std::memory_order_relaxed);
+  return n;
+}
+template <int BN, bool PAIR>
+static int wgrad_at_once(int cluster) {
+  static std::atomic<int> known[64][9];
+  return clusters_at_once(mx_weight_grad_kernel<BN, PAIR>, known, kWgradThreads, WgradSmem<BN, PAIR>::kBytes, cluster);
+}
+
 template <int BN, bool PAIR>
 static int run_wgrad(const CUtensorMap& codes, const CUtensorMap& grad, const WgradArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
   const int cluster = a.splits * (PAIR ? 2 : 1);
-  return launch_tc(mx_weight_grad_kernel<BN, PAIR>, raised, WgradSmem<BN, PAIR>::kBytes, (int64_t)a.k_tiles * a.n_tiles * cluster, cluster, st, codes, grad, a);
+  return launch_tc(mx_weight_grad_kernel<BN, PAIR>, raised, kWgradThreads, WgradSmem<BN, PAIR>::kBytes, (int64_t)a.k_tiles * a.n_tiles * cluster, cluster, st, codes, grad, a);
 }
 
 template <int BN>
 static int run_fp4(const CUtensorMap& ma, const CUtensorMap& mb, const Fp4Args& a, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
-  return launch_tc(mx_fp4_kernel<BN>, raised, Fp4Smem<BN>::kBytes, (int64_t)a.n_tiles * a.m_tiles * a.splits, a.splits, st, ma, mb, a);
+  return launch_tc(mx_fp4_kernel<BN>, raised, kFp4Threads, Fp4Smem<BN>::kBytes, (int64_t)a.n_tiles * a.m_tiles * a.splits, a.splits, st, ma, mb, a);
 }
 
 static int pieces_of(int dtype) { return dtype == RT_F32 ? 3 : dtype == RT_F16 ? 2 : 1; }
@@ -579,20 +675,24 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   a.tokens = (int)tokens;
   a.token_steps = (int)((tokens + kTok - 1) / kTok);
   a.pieces = pieces;
-  a.out = {out, ld_out, (int)n, (int)k, out_dtype, accumulate != 0};
+  a.out = {out, ld_out, (int)n, (int)k, out_dtype, accumulate != 0, aligned16(out, ld_out, dtype_size(out_dtype))};
 
-  // Tile and split.  A step costs what the longest of product, conversion and loads costs; a CTA
-  // also pays for its start, its output and, when split, the exchange (clocks, measured).
+  // Tile and split: the fewest nanoseconds, counted as rounds of clusters that run together times
+  // (steps times what a step takes with this tile + start and output + the exchange when split), all measured.
   const int64_t steps = (int64_t)a.token_steps * pieces;
-  struct Shape { int bn, ctas; double step; };
-  static const Shape shapes[] = {{512, 2, 1100}, {256, 2, 650}, {128, 1, 500}, {64, 1, 400}};
+  struct Shape { int bn, ctas; double step, fixed; int (*at_once)(int); };
+  static const Shape shapes[] = {{512, 2, 560, 6000, wgrad_at_once<512, true>},
+                                 {256, 2, 400, 5000, wgrad_at_once<256, true>},
+                                 {128, 1, 380, 4500, wgrad_at_once<128, false>},
+                                 {64, 1, 360, 4000, wgrad_at_once<64, false>}};
   const Shape* pick = nullptr;
   double best = 1e300;
   for (const Shape& c : shapes)
-    for (int s = 1; s * c.ctas <= 8; s *= 2) {
+    for (int s = 1; s * c.ctas <= 8; ++s) {
       if (s > steps || (s > 1 && c.bn > 256)) continue;      // a split tile has to fit into shared memory
-      const int64_t ctas = (k + 128 * c.ctas - 1) / (128 * c.ctas) * c.ctas * ((n + c.bn - 1) / c.bn) * s;
-      const double cost = (double)((ctas + kSms - 1) / kSms) * ((double)((steps + s - 1) / s) * c.step + 3000 + c.bn * 12 + (s > 1 ? 2500 : 0));
+      const int64_t tiles = (k + 128 * c.ctas - 1) / (128 * c.ctas) * ((n + c.bn - 1) / c.bn);
+      const int at_once = c.at_once(s * c.ctas);
+      const double cost = (double)((tiles + at_once - 1) / at_once) * ((double)((steps + s - 1) / s) * c.step + c.fixed + (s > 1 ? 2000 : 0));
       if (cost < best) { best = cost; pick = &c; a.splits = s; }
     }
   a.k_tiles = (int)((k + 128 * pick->ctas - 1) / (128 * pick->ctas));
@@ -653,7 +753,7 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
   a.k_padded = (int)kp;
   a.steps = (int)((kp + kStepK - 1) / kStepK);
   a.ktiles = (int)((kp + 127) / 128);
-  a.out = {out, ld_out, (int)m, (int)n, out_dtype, 0};
+  a.out = {out, ld_out, (int)m, (int)n, out_dtype, 0, aligned16(out, ld_out, dtype_size(out_dtype))};
 
   const int64_t n_tiles = (n + 127) / 128;
   int bm = 128, splits = 1;
