@@ -26,6 +26,8 @@ constexpr int kFirstWorker = 4;          // warp 0: loads, 1: products, 2: tenso
 constexpr int kConvGroups = 2;           // of four warps each, in the weight gradient's kernel
 constexpr int kWgradThreads = 32 * (kFirstWorker + 4 * kConvGroups);
 constexpr int kFp4Threads = 32 * (kFirstWorker + 8);
+constexpr int kPairGroups = 2;           // of four output warps each
+constexpr int kPairThreads = 32 * (kFirstWorker + 4 * kPairGroups);
 
 struct OutMatrix {
   void* p;
@@ -66,28 +68,16 @@ __device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col
 }
 
 // 32 columns of the accumulator, from this warp's quarter of the lanes, as 32 output rows of 32 values:
-// through 32 x 32 values of shared memory that the warp has to itself, so that a lane stores 16 bytes
-// of one row.  Straight from the registers, 64 bytes of one row to a warp, a column of a tile took 17 ns, this
-// way 8; TMA stores from shared memory were no faster.
+// through 2 KB of shared memory that the warp has to itself (fp32 in two halves), so that a lane stores 16
+// bytes of one row.  Straight from the registers, 64 bytes of one row to a warp, a column of a tile took
+// 17 ns, this way 8; TMA stores from shared memory were no faster.
 template <int D>
-__device__ __forceinline__ void put_square(const OutMatrix& o, uint32_t tmem, int row, int col, elem_t<D>* room) {
-  constexpr int kLanes = D == RT_F32 ? 8 : 4, kPer = 32 / kLanes;     // lanes to a row, values to a lane
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void put_room(const OutMatrix& o, int row, int col, const elem_t<D>* room) {
+  constexpr int kLanes = D == RT_F32 ? 8 : 4, kPer = 16 / (int)sizeof(elem_t<D>), kRows = 32 / kLanes;   // lanes to a row, values to a lane, rows to a store
+  const int lane = threadIdx.x & 31, c = col + lane % kLanes * kPer;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t acc[16];
-    tmem_load16(tmem + 16 * h, acc);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if constexpr (D == RT_F32) room[(16 * h + j) * 32 + lane] = __uint_as_float(acc[j]);
-      else room[(16 * h + j) * 32 + lane] = of_f32<D>(__uint_as_float(acc[j]));
-    }
-  }
-  __syncwarp();
-  const int c = col + lane % kLanes * kPer;
-#pragma unroll
-  for (int i = 0; i < kLanes; ++i) {
-    const int r = i * kPer + lane / kLanes;
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * kRows + lane / kLanes;
     if (row + r < o.rows && c < o.cols) {
       const uint4 v = *reinterpret_cast<const uint4*>(room + r * 32 + lane % kLanes * kPer);
       elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + (int64_t)(row + r) * o.ld + c;
@@ -100,7 +90,25 @@ __device__ __forceinline__ void put_square(const OutMatrix& o, uint32_t tmem, in
       }
     }
   }
-  __syncwarp();
+}
+template <int D>
+__device__ __forceinline__ void put_square(const OutMatrix& o, uint32_t tmem, int row, int col, elem_t<D>* room) {
+  const int lane = threadIdx.x & 31;
+  uint32_t acc[2][16];
+  tmem_load16(tmem, acc[0]);
+  tmem_load16(tmem + 16, acc[1]);
+  tmem_wait(acc[0]);
+  tmem_wait(acc[1]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) room[((D == RT_F32 ? 0 : 16 * h) + j) * 32 + lane] = of_f32<D>(__uint_as_float(acc[h][j]));
+    if (D == RT_F32 || h == 1) {
+      __syncwarp();
+      put_room<D>(o, D == RT_F32 ? row + 16 * h : row, col, room);
+      __syncwarp();
+    }
+  }
 }
 
 // The worker warps' part after the last product.  One CTA per tile: straight from tensor memory.
@@ -121,7 +129,7 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
         if (splits == 1) {
           if (row0 + c >= o.rows) break;
           if (o.wide && !o.accumulate) {
-            float* room = parts + (warp - kFirstWorker) * 1024;
+            float* room = parts + (warp - kFirstWorker) * 512;
             if (o.dtype == RT_BF16) put_square<RT_BF16>(o, lanes + c, row0 + c, col0 + q * 32, reinterpret_cast<uint16_t*>(room));
             else if (o.dtype == RT_F32) put_square<RT_F32>(o, lanes + c, row0 + c, col0 + q * 32, room);
             else put_square<RT_F16>(o, lanes + c, row0 + c, col0 + q * 32, reinterpret_cast<uint16_t*>(room));
@@ -132,6 +140,7 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
         for (int h = 0; h < 2; ++h) {
           uint32_t acc[16];
           tmem_load16(lanes + c + 16 * h, acc);
+          tmem_wait(acc);
           if (splits == 1) {
             if (o.dtype == RT_BF16) put_columns<RT_BF16>(o, row0 + c + 16 * h, col0 + q * 32 + lane, acc);
             else if (o.dtype == RT_F32) put_columns<RT_F32>(o, row0 + c + 16 * h, col0 + q * 32 + lane, acc);
@@ -495,12 +504,12 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
         const uint32_t sf = tmem + BN + 16 * s;
         const int halves = min(2, a.ktiles - 2 * it), products = min(4, (a.k_padded - it * kStepK + 63) / 64);
         for (int h = 0; h < halves; ++h) {
-          copy_scales(sf + 4 * h, plain_desc(scale_b + s * S::kScale + 512 * h, 128, 128));
-          copy_scales(sf + 8 + 4 * h, plain_desc(scale_a + s * S::kScale + 512 * h, 128, 128));
+          copy_scales<false>(sf + 4 * h, plain_desc(scale_b + s * S::kScale + 512 * h, 128, 128));
+          copy_scales<false>(sf + 8 + 4 * h, plain_desc(scale_a + s * S::kScale + 512 * h, 128, 128));
         }
         const uint64_t db = tile_desc(tile_b + s * S::kA, 16, 1024), da = tile_desc(tile_a + s * S::kB, 16, 1024);
         for (int kk = 0; kk < products; ++kk)
-          mma_mxfp4(tmem, db + kk * 2, da + kk * 2, kk & 1 ? idesc_mxfp4(128, BN, 1) : idesc_mxfp4(128, BN, 0), sf + 4 * (kk >> 1),
+          mma_mxfp4<false>(tmem, db + kk * 2, da + kk * 2, kk & 1 ? idesc_mxfp4(128, BN, 1) : idesc_mxfp4(128, BN, 0), sf + 4 * (kk >> 1),
                     sf + 8 + 4 * (kk >> 1), i > 0 || kk > 0);
         tc_commit<false>(empty + 8 * s);
       }
@@ -515,6 +524,159 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
   finish_tile<BN, 8>(a.out, tmem, m0, n0, a.splits, 0, 1, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
   if (warp == 2) tmem_free<false>(tmem, S::kColumns);
+}
+
+// Large products: pairs of CTAs stay and take tile after tile, 256 rows of b (128 to a CTA) x 384 rows of a
+// (192 to a CTA), as a product of 256 columns and one of 128 per 64 columns of the sum.  What bounds
+// the small tiles above is the way from L2: 34 KB per CTA for 256 clocks of products at 128 x 128,
+// here 44 KB for 768.  384 columns of sums and four stages of scales (8 columns of b's, 24 of a's) fill
+// tensor memory, so a tile's output is not overlapped with the next one's products, but its loads are.
+// Every CTA needs the scales of all 384 rows of a.  Both CTAs' loads report to the first one's barrier (told
+// by a warp of the second instead, a step took 550 ns); the first issues all copies and products.
+struct PairSmem {
+  static constexpr int kLanes = 128 * 128, kRows1 = 128 * 128, kRows2 = 64 * 128, kLaneScales = 1024, kRowScales = 3 * 1024;
+  static constexpr int kStage = kLanes + kRows1 + kRows2 + kLaneScales + kRowScales;
+  static constexpr int kStages = 4, kRoom = 4 * kPairGroups * 2048;
+  static constexpr int kBytes = kStages * kStage + kRoom + 1024 + 256;
+  static constexpr int kTileRows = 384, kSums = 384, kScaleColumns = 32;
+};
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+mx_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb, const Fp4Args a) {
+  using S = PairSmem;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t tile_b = base, tile_a1 = tile_b + S::kStages * S::kLanes, tile_a2 = tile_a1 + S::kStages * S::kRows1;
+  const uint32_t scale_b = tile_a2 + S::kStages * S::kRows2, scale_a = scale_b + S::kStages * S::kLaneScales;
+  const uint32_t room = scale_a + S::kStages * S::kRowScales, bars = room + S::kRoom;
+  const uint32_t full = bars, empty = full + 8 * S::kStages, done = empty + 8 * S::kStages, drained = done + 8, slot = drained + 8;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, side = blockIdx.x & 1;
+  const int tiles = a.n_tiles * a.m_tiles, pairs = gridDim.x >> 1;
+
+  if (warp == 0 && elect_one()) {
+    prefetch_map(&map_a1);
+    prefetch_map(&map_a2);
+    prefetch_map(&map_b);
+    prefetch_map(&map_sa);
+    prefetch_map(&map_sb);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full + 8 * s, 1);            // the first CTA's: expects both CTAs' bytes
+      mbar_init(empty + 8 * s, 1);
+    }
+    mbar_init(done, 1);
+    mbar_init(drained, 2 * 4 * kPairGroups); // the output warps of both CTAs
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc<true>(slot, 512);
+  __syncthreads();
+  cluster_sync();                            // the other CTA's barriers are there
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + (slot - base));
+  bool ok = true;
+
+  // tile t: eight tiles of a's rows side by side, b's inside
+  auto place = [&](int t, int& m0, int& n0) {
+    const int per_group = 8 * a.n_tiles, group = t / per_group, width = min(8, a.m_tiles - 8 * group), in = t - group * per_group;
+    m0 = (group * 8 + in % width) * S::kTileRows;
+    n0 = in / width * 256;
+  };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int i = 0;                             // steps so far, over all tiles
+      for (int t = blockIdx.x >> 1; t < tiles && ok; t += pairs) {
+        int m0, n0;
+        place(t, m0, n0);
+        const int row = n0 + side * 128;
+        for (int k = 0; k < a.steps; ++k, ++i) {
+          const int s = i % S::kStages;
+          if (!(ok = mbar_wait(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
+          if (side == 0) mbar_expect(full + 8 * s, 2 * S::kStage);
+          const uint32_t bar = address_at(full + 8 * s, 0);
+          tma_load_2d_pair(&map_b, tile_b + s * S::kLanes, bar, k * 128, row);
+          tma_load_2d_pair(&map_a1, tile_a1 + s * S::kRows1, bar, k * 128, m0 + side * 128);
+          tma_load_2d_pair(&map_a2, tile_a2 + s * S::kRows2, bar, k * 128, m0 + 256 + side * 64);
+          tma_load_2d_pair(&map_sb, scale_b + s * S::kLaneScales, bar, k * 256, row >> 7);
+          tma_load_2d_pair(&map_sa, scale_a + s * S::kRowScales, bar, k * 256, m0 >> 7);
+        }
+      }
+      // If a wait ran out, loads may still be on their way to both CTAs' memory; all of them report to the first CTA's
+      // barriers, which it waits for (again with the limit) before the pair's last barrier lets either end.
+      if (!ok && side == 0)
+        for (int j = 0; j < S::kStages && j < i; ++j) {
+          const int latest = i - 1 - (i - 1 - j) % S::kStages;
+          mbar_wait(full + 8 * j, (latest / S::kStages) & 1);
+        }
+    }
+  } else if (warp == 1) {
+    if (side == 0 && elect_one()) {
+      int i = 0, n = 0;
+      for (int t = blockIdx.x >> 1; t < tiles && ok; t += pairs, ++n) {
+        if (n > 0 && !(ok = mbar_wait(drained, (n - 1) & 1))) break;
+        for (int k = 0; k < a.steps; ++k, ++i) {
+          const int s = i % S::kStages;
+          if (!(ok = mbar_wait(full + 8 * s, (i / S::kStages) & 1))) break;
+          tc_fence_after();
+          const uint32_t sf = tmem + S::kSums + S::kScaleColumns * s;
+          const int halves = min(2, a.ktiles - 2 * k), products = min(4, (a.k_padded - k * kStepK + 63) / 64);
+          for (int h = 0; h < halves; ++h) {
+            copy_scales<true>(sf + 4 * h, plain_desc(scale_b + s * S::kLaneScales + 512 * h, 128, 128));
+#pragma unroll
+            for (int r = 0; r < 3; ++r)
+              copy_scales<true>(sf + 8 + 12 * h + 4 * r, plain_desc(scale_a + s * S::kRowScales + 1024 * r + 512 * h, 128, 128));
+          }
+          const uint64_t db = tile_desc(tile_b + s * S::kLanes, 16, 1024), d1 = tile_desc(tile_a1 + s * S::kRows1, 16, 1024), d2 = tile_desc(tile_a2 + s * S::kRows2, 16, 1024);
+          for (int kk = 0; kk < products; ++kk) {
+            const uint32_t sb = sf + 4 * (kk >> 1), sa = sf + 8 + 12 * (kk >> 1);
+            mma_mxfp4<true>(tmem, db + kk * 2, d1 + kk * 2, kk & 1 ? idesc_mxfp4(256, 256, 1) : idesc_mxfp4(256, 256, 0), sb, sa, k > 0 || kk > 0);
+            mma_mxfp4<true>(tmem + 256, db + kk * 2, d2 + kk * 2, kk & 1 ? idesc_mxfp4(256, 128, 1) : idesc_mxfp4(256, 128, 0), sb, sa + 8, k > 0 || kk > 0);
+          }
+          tc_commit<true>(empty + 8 * s, 3);
+        }
+        tc_commit<true>(done, 3);
+      }
+    }
+  } else if (warp >= kFirstWorker) {
+    const int q = warp & 3, group = (warp - kFirstWorker) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+    float* space = reinterpret_cast<float*>(smem + (room - base)) + (warp - kFirstWorker) * 512;
+    int n = 0;
+    for (int t = blockIdx.x >> 1; t < tiles; t += pairs, ++n) {
+      int m0, n0;
+      place(t, m0, n0);
+      if (!(ok = mbar_wait(done, n & 1))) break;
+      tc_fence_after();
+      const int col = n0 + side * 128 + q * 32;
+#pragma unroll 1
+      for (int c = group * 32; c < S::kTileRows && m0 + c < a.out.rows; c += 32 * kPairGroups) {
+        if (a.out.wide) {
+          if (a.out.dtype == RT_BF16) put_square<RT_BF16>(a.out, lanes + c, m0 + c, col, reinterpret_cast<uint16_t*>(space));
+          else if (a.out.dtype == RT_F32) put_square<RT_F32>(a.out, lanes + c, m0 + c, col, space);
+          else put_square<RT_F16>(a.out, lanes + c, m0 + c, col, reinterpret_cast<uint16_t*>(space));
+          continue;
+        }
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t acc[16];
+          tmem_load16(lanes + c + 16 * h, acc);
+          tmem_wait(acc);
+          if (a.out.dtype == RT_BF16) put_columns<RT_BF16>(a.out, m0 + c + 16 * h, col + lane, acc);
+          else if (a.out.dtype == RT_F32) put_columns<RT_F32>(a.out, m0 + c + 16 * h, col + lane, acc);
+          else put_columns<RT_F16>(a.out, m0 + c + 16 * h, col + lane, acc);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_at(drained, 0);
+    }
+  }
+  __syncwarp();
+  if (!ok) atomicAdd(&g_wait_faults, 1u);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                            // the products read both CTAs' memory, the barriers are in both
+  if (warp == 2) tmem_free<true>(tmem, 512);
 }
 
 static int check_out(const void* out, int dtype, int64_t cols, int64_t ld) {
@@ -563,6 +725,7 @@ static int launch_tc(K kernel, std::atomic<uint64_t>& raised, int threads, int s
   RT_CUDA(cudaGetDevice(&device));
   if (device >= 64 || !(raised.load(std::memory_order_acquire) >> device & 1)) {
     RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    RT_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     if (device < 64) raised.fetch_or(1ull << device, std::memory_order_release);
   }
   cudaLaunchConfig_t cfg{};
@@ -602,6 +765,7 @@ static int clusters_at_once(K kernel, std::atomic<int> (&known)[64][9], int thre
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
     return std::max(1, kSms / cluster);
@@ -626,6 +790,16 @@ template <int BN>
 static int run_fp4(const CUtensorMap& ma, const CUtensorMap& mb, const Fp4Args& a, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
   return launch_tc(mx_fp4_kernel<BN>, raised, kFp4Threads, Fp4Smem<BN>::kBytes, (int64_t)a.n_tiles * a.m_tiles * a.splits, a.splits, st, ma, mb, a);
+}
+
+template <int BN>
+static int fp4_at_once(int cluster) {
+  static std::atomic<int> known[64][9];
+  return clusters_at_once(mx_fp4_kernel<BN>, known, kFp4Threads, Fp4Smem<BN>::kBytes, cluster);
+}
+static int fp4_pairs_at_once() {
+  static std::atomic<int> known[64][9];
+  return clusters_at_once(mx_fp4_pair_kernel, known, kPairThreads, PairSmem::kBytes, 2);
 }
 
 static int pieces_of(int dtype) { return dtype == RT_F32 ? 3 : dtype == RT_F16 ? 2 : 1; }
@@ -755,17 +929,27 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
   a.ktiles = (int)((kp + 127) / 128);
   a.out = {out, ld_out, (int)m, (int)n, out_dtype, 0, aligned16(out, ld_out, dtype_size(out_dtype))};
 
+  // Tile and split, by the microseconds that were measured for each: a start, then rounds of what runs
+  // together.  Unsplit tiles run two to an SM and slow each other down; clusters run one CTA to an SM.
+  // (8192 x 11008 x 4096: 208 us in 128 x 128 tiles, 154 in pairs; 2048 x 4096 x 4096: 24 and 27; 1 x 4096 x 4096:
+  // 8.9 unsplit, 6.4 in four.)
   const int64_t n_tiles = (n + 127) / 128;
-  int bm = 128, splits = 1;
+  const int width = m <= 32 ? 32 : m <= 64 ? 64 : 128;      // rows of a to a tile: narrow ones only for a single tile
+  const int64_t tiles = n_tiles * ((m + width - 1) / width);
+  int bm = width, splits = 1;
   double best = 1e300;
-  for (const int width : {128, 64, 32})
-    for (const int s : {1, 2, 4, 8}) {
-      if (s > a.steps || (width < 128 && m > width)) continue;
-      const double step = width == 128 ? 450 : width == 64 ? 300 : 250;
-      const int64_t ctas = n_tiles * ((m + width - 1) / width) * s;
-      const double cost = (double)((ctas + 2 * kSms - 1) / (2 * kSms)) * ((double)((a.steps + s - 1) / s) * step + 2000 + width * 12 + (s > 1 ? 1500 : 0));
-      if (cost < best) { best = cost; bm = width; splits = s; }
-    }
+  for (int s = 1; s <= 8 && s <= a.steps; ++s) {
+    const int at_once = s == 1 ? 2 * kSms : width == 128 ? fp4_at_once<128>(s) : width == 64 ? fp4_at_once<64>(s) : fp4_at_once<32>(s);
+    const double step = s > 1 ? 0.34 : 0.34 + 0.26 * std::min(1.0, std::max(0.0, (double)(tiles - kSms) / kSms));
+    const double cost = 4.0 + (s > 1 ? 1.5 : 0) + (double)((tiles + at_once - 1) / at_once) * ((double)((a.steps + s - 1) / s) * step + (s > 1 ? 1.0 : 1.5)) - 1.5;
+    if (cost < best) { best = cost; splits = s; }
+  }
+  const int64_t pair_tiles = (n + 255) / 256 * ((m + 383) / 384);
+  if (pair_tiles > 0x3FFFFFFFll) return fail(RT_E_SIZE, "m * n is too large");
+  if (m > 128) {
+    const int at_once = fp4_pairs_at_once();
+    if (3.5 + (double)((pair_tiles + at_once - 1) / at_once) * (a.steps * 0.58 + 2.2) < best) bm = 384;
+  }
   a.splits = splits;
   a.n_tiles = (int)n_tiles;
   a.m_tiles = (int)((m + bm - 1) / bm);
@@ -775,13 +959,29 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
   const uint64_t strides[1] = {(uint64_t)kp / 2};
   {
     const uint64_t dims[2] = {(uint64_t)kp / 2, (uint64_t)m};
-    const uint32_t box[2] = {128, (uint32_t)bm};
+    const uint32_t box[2] = {128, (uint32_t)std::min(bm, 128)};
     if (int rc = make_map(&map_a, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   }
   {
     const uint64_t dims[2] = {(uint64_t)kp / 2, (uint64_t)n};
     const uint32_t box[2] = {128, 128};
     if (int rc = make_map(&map_b, CU_TENSOR_MAP_DATA_TYPE_UINT8, b_codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  }
+  if (bm == 384) {
+    CUtensorMap map_a2;
+    const uint64_t dims[2] = {(uint64_t)kp / 2, (uint64_t)m};
+    const uint32_t box[2] = {128, 64};
+    if (int rc = make_map(&map_a2, CU_TENSOR_MAP_DATA_TYPE_UINT8, a_codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    // the scales as rows of tiles, in words: a box is the two tiles of a step, of one or of three row tiles
+    CUtensorMap map_sa, map_sb;
+    const uint64_t wide[1] = {(uint64_t)a.ktiles * 512};
+    const uint64_t dims_a[2] = {(uint64_t)a.ktiles * 128, (uint64_t)(m + 127) / 128}, dims_b[2] = {(uint64_t)a.ktiles * 128, (uint64_t)n_tiles};
+    const uint32_t box_a[2] = {256, 3}, box_b[2] = {256, 1};
+    if (int rc = make_map(&map_sa, CU_TENSOR_MAP_DATA_TYPE_UINT32, a_scales, 2, dims_a, wide, box_a, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    if (int rc = make_map(&map_sb, CU_TENSOR_MAP_DATA_TYPE_UINT32, b_scales, 2, dims_b, wide, box_b, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+    static std::atomic<uint64_t> raised{0};
+    a.n_tiles = (int)((n + 255) / 256);
+    return launch_tc(mx_fp4_pair_kernel, raised, kPairThreads, PairSmem::kBytes, 2 * std::min<int64_t>(pair_tiles, fp4_pairs_at_once()), 2, st, map_a, map_a2, map_b, map_sa, map_sb, a);
   }
   if (bm == 128) return run_fp4<128>(map_a, map_b, a, st);
   if (bm == 64) return run_fp4<64>(map_a, map_b, a, st);

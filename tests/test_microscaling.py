@@ -619,7 +619,8 @@ def test_weight_gradient_of_many_tiles(tokens, n, k):
 
 
 @gpu
-@pytest.mark.parametrize("m,n,k", [(129, 300, 700), (700, 2100, 512), (2000, 500, 1024), (320, 4000, 300), (1, 20000, 4096), (60, 5000, 2080)])
+@pytest.mark.parametrize("m,n,k", [(129, 300, 700), (700, 2100, 512), (2000, 500, 1024), (320, 4000, 300), (1, 20000, 4096), (60, 5000, 2080), (384, 256, 256),
+                                   (385, 257, 1300), (3000, 9000, 160), (1000, 20000, 4100)])
 def test_fp4_product_of_many_tiles(m, n, k):
     a = mx.quantize_mxfp4(U.matrix(m, k, "bf16", 17, 1.0, DEV))
     b = mx.quantize_mxfp4(U.matrix(n, k, "bf16", 18, 0.02, DEV))
