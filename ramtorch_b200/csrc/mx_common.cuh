@@ -126,6 +126,86 @@ __device__ __forceinline__ void store_raw(void* base, int64_t i, const Raw8<D>& 
   if constexpr (D == RT_F32) q[1] = r.w[1];
 }
 
+struct Matrix {            // rows x cols, row stride ld elements
+  const void* p;
+  int64_t ld;
+};
+
+// the 16 bytes from byte `off` (even, below 16) of the 32 bytes a, b
+__device__ __forceinline__ uint4 cut16(const uint4& a, const uint4& b, uint32_t off) {
+  const bool two = off & 8u, one = off & 4u;
+  const uint32_t t0 = two ? a.z : a.x, t1 = two ? a.w : a.y, t2 = two ? b.x : a.z, t3 = two ? b.y : a.w, t4 = two ? b.z : b.x, t5 = two ? b.w : b.y;
+  const uint32_t v0 = one ? t1 : t0, v1 = one ? t2 : t1, v2 = one ? t3 : t2, v3 = one ? t4 : t3, v4 = one ? t5 : t4;
+  const uint32_t sh = (off & 3u) * 8;
+  return make_uint4(__funnelshift_r(v0, v1, sh), __funnelshift_r(v1, v2, sh), __funnelshift_r(v2, v3, sh), __funnelshift_r(v3, v4, sh));
+}
+
+// The unit at p, column c of its row; columns beyond the last are 0.  VEC: every row starts on a
+// 16-byte boundary.  Otherwise a unit that has a whole unit before it and 16 bytes of its row behind
+// it is cut out of aligned chunks, which then lie inside the row.
+template <int D, bool VEC>
+__device__ __forceinline__ Raw8<D> load_unit(const elem_t<D>* p, const int c, const int cols, const bool live) {
+  constexpr int kSize = sizeof(elem_t<D>);
+  Raw8<D> raw{};
+  if (!live) return raw;
+  const uint32_t off = VEC ? 0u : (uint32_t)(uintptr_t)p & 15u;
+  if ((VEC || off == 0) && c + 8 <= cols) {
+    raw = load_raw<D>(p, 0);
+  } else if (!VEC && c >= 8 && c + 8 + 16 / kSize <= cols) {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) - off);
+    const uint4 a = __ldg(q), b = __ldg(q + 1);
+    raw.w[0] = cut16(a, b, off);
+    if constexpr (D == RT_F32) raw.w[1] = cut16(b, __ldg(q + 2), off);
+  } else if (c < cols) {
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = c + k < cols ? to_f32<D>(p[k]) : 0.f;
+    raw = pack<D>(x);   // exact: the values are of this type
+  }
+  return raw;
+}
+// The units of a thread.  Where none of them needs a second look, which is nearly always, all loads
+// are issued before the first is used; a unit that may come in pieces would be waited for.
+template <int D, bool VEC, int R>
+__device__ __forceinline__ void load_units(const elem_t<D>* const (&p)[R], const int (&c)[R], const bool (&live)[R], const int cols, Raw8<D> (&raw)[R]) {
+  constexpr int kSize = sizeof(elem_t<D>), kWords = D == RT_F32 ? 2 : 1;
+  bool inner = true;
+#pragma unroll
+  for (int k = 0; k < R; ++k) inner = inner && live[k] && (VEC ? c[k] + 8 <= cols : c[k] >= 8 && c[k] + 8 + 16 / kSize <= cols);
+  if (inner) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) raw[k] = load_raw<D>(p[k], 0);
+    } else {
+      uint4 chunk[R][kWords + 1];
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int j = 0; j <= kWords; ++j) chunk[k][j] = __ldg(reinterpret_cast<const uint4*>((uintptr_t)p[k] & ~(uintptr_t)15) + j);
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int j = 0; j < kWords; ++j) raw[k].w[j] = cut16(chunk[k][j], chunk[k][j + 1], (uint32_t)(uintptr_t)p[k] & 15u);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < R; ++k) raw[k] = load_unit<D, VEC>(p[k], c[k], cols, live[k]);
+  }
+}
+// of rows `step` apart
+template <int D, bool VEC, int R>
+__device__ __forceinline__ void load_rows(const Matrix& m, int64_t row, int step, int c, int cols, int64_t rows, Raw8<D> (&raw)[R]) {
+  const elem_t<D>* p[R];
+  int cs[R];
+  bool live[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    p[k] = static_cast<const elem_t<D>*>(m.p) + (row + k * step) * m.ld + c;
+    cs[k] = c;
+    live[k] = row + k * step < rows;
+  }
+  load_units<D, VEC, R>(p, cs, live, cols, raw);
+}
 inline bool aligned16(const void* p, int64_t ld, int size) {
   return (((uintptr_t)p) & 15) == 0 && (ld * size) % 16 == 0;
 }

@@ -389,28 +389,51 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
 // A gradient that the tensor maps cannot take as it is (fp32, fp16, rows that do not start on 16-byte
 // boundaries) as bf16 planes whose sum it is: the leading 8 bits of each value's mantissa, the next 8,
 // the rest.  Cut, not rounded, so that nothing overflows; an infinity or a NaN is in the first plane alone.
-template <int D, int P>
+// Eight values of a row to a thread, of two rows, planes of np = n rounded up to eight columns.
+template <int D, int P, bool VEC>
 __global__ void __launch_bounds__(256)
-spread_gradient_kernel(const elem_t<D>* __restrict__ g, const int64_t ld, const int64_t tokens, const int n, const int np, uint16_t* __restrict__ planes) {
-  const int64_t total = tokens * np;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / np;
-    const int c = (int)(i - t * np);
-    float v = c < n ? to_f32<D>(g[t * ld + c]) : 0.f;
+spread_gradient_kernel(const Matrix g, const FastDiv upr, const int64_t tokens, const int n, uint16_t* __restrict__ planes) {
+  uint32_t group, c8;
+  upr.split(blockIdx.x * 256 + threadIdx.x, group, c8);
+  const int64_t row = (int64_t)group * 2, total = tokens * upr.d * 8;
+  Raw8<D> raw[2];
+  load_rows<D, VEC>(g, row, 1, (int)c8 * 8, n, tokens, raw);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    if (row + r >= tokens) break;
+    uint16_t* out = planes + (row + r) * upr.d * 8 + c8 * 8;
     if constexpr (P == 1) {
-      planes[i] = of_f32<RT_BF16>(v);
+      *reinterpret_cast<uint4*>(out) = raw[r].w[0];
     } else {
-      uint32_t b = __float_as_uint(v);
-      const bool odd = (b & 0x7F800000u) == 0x7F800000u;
-      if (odd && (b & 0x7FFFFFu)) b = 0x7FC00000u;
+      float v[8];
+      unpack<D>(raw[r], v);
+      uint32_t b[8];
+      bool odd[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        b[k] = __float_as_uint(v[k]);
+        odd[k] = (b[k] & 0x7F800000u) == 0x7F800000u;
+        if (odd[k] && (b[k] & 0x7FFFFFu)) b[k] = 0x7FC00000u;
+      }
 #pragma unroll
       for (int p = 0; p < P; ++p) {
-        planes[p * total + i] = (uint16_t)(b >> 16);
-        v = odd ? 0.f : v - __uint_as_float(b & 0xFFFF0000u);
-        b = __float_as_uint(v);
+        *reinterpret_cast<uint4*>(out + p * total) = make_uint4(__byte_perm(b[0], b[1], 0x7632), __byte_perm(b[2], b[3], 0x7632),
+                                                                __byte_perm(b[4], b[5], 0x7632), __byte_perm(b[6], b[7], 0x7632));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          v[k] = odd[k] ? 0.f : v[k] - __uint_as_float(b[k] & 0xFFFF0000u);
+          b[k] = __float_as_uint(v[k]);
+        }
       }
     }
   }
+}
+template <int D, int P>
+static void run_spread(const void* g, int64_t ld, int64_t tokens, int64_t n, void* planes, cudaStream_t st) {
+  const FastDiv upr = FastDiv::of((uint32_t)((n + 7) / 8));
+  const unsigned nb = (unsigned)(((uint64_t)((tokens + 1) / 2) * upr.d + 255) / 256);
+  auto k = aligned16(g, ld, (int)sizeof(elem_t<D>)) ? spread_gradient_kernel<D, P, true> : spread_gradient_kernel<D, P, false>;
+  k<<<nb, 256, 0, st>>>({g, ld}, upr, tokens, (int)n, (uint16_t*)planes);
 }
 
 // ---------------------------------------------------------------------------------- fp4 product
@@ -886,10 +909,9 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
     if (int rc = make_map(&map_grad, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, need ? workspace : grad_out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   }
   if (need) {
-    const unsigned nb = (unsigned)std::min<int64_t>((tokens * np + 255) / 256, kSms * 16);
-    if (grad_dtype == RT_F32) spread_gradient_kernel<RT_F32, 3><<<nb, 256, 0, st>>>((const float*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
-    else if (grad_dtype == RT_F16) spread_gradient_kernel<RT_F16, 2><<<nb, 256, 0, st>>>((const uint16_t*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
-    else spread_gradient_kernel<RT_BF16, 1><<<nb, 256, 0, st>>>((const uint16_t*)grad_out, ld_grad, tokens, (int)n, (int)np, (uint16_t*)workspace);
+    if (grad_dtype == RT_F32) run_spread<RT_F32, 3>(grad_out, ld_grad, tokens, n, workspace, st);
+    else if (grad_dtype == RT_F16) run_spread<RT_F16, 2>(grad_out, ld_grad, tokens, n, workspace, st);
+    else run_spread<RT_BF16, 1>(grad_out, ld_grad, tokens, n, workspace, st);
     if (int rc = launched()) return rc;
   }
   if (pick->bn == 512) return run_wgrad<512, true>(map_codes, map_grad, a, st);
