@@ -16,17 +16,27 @@ from . import helpers
 from . import microscaling as mx
 
 
+def _rowed(t: torch.Tensor) -> torch.Tensor:
+    """`t` itself where its rows are evenly spaced runs of memory, else a copy that is."""
+    try:
+        mx._rows(t, "t")
+        return t
+    except ValueError:
+        return t.contiguous()
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, product, seed, tensor_id, step):
+        x = _rowed(x)
         w = weight if weight.is_cuda else weight.detach().to(x.device, non_blocking=True)
         if product == "mxfp4":
-            y = mx.mxfp4_matmul(mx.quantize_mxfp4(x), mx.quantize_mxfp4(w), dtype=x.dtype)
+            y = mx.mxfp4_matmul(mx.quantize_mxfp4(x), mx.quantize_mxfp4(_rowed(w)), dtype=x.dtype)
         else:
             y = x @ w.t()
         if bias is not None:
             y = y + bias.to(x.device)
-        keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] or not weight.is_cuda and weight.requires_grad else None
+        keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(*((keep.codes, keep.scales) if keep is not None else (None, None)), weight)
         ctx.x_shape, ctx.x_dtype, ctx.args = tuple(x.shape), x.dtype, (product, seed, tensor_id, step)
         ctx.bias_like = None if bias is None else {"dtype": bias.dtype, "device": bias.device}
@@ -37,13 +47,13 @@ class _Linear(torch.autograd.Function):
     def backward(ctx, grad):
         codes, scales, weight = ctx.saved_tensors
         product, seed, tensor_id, step = ctx.args
-        grad = grad if grad.is_contiguous() else grad.contiguous()
+        grad = _rowed(grad)
         gx = gw = gb = None
         if ctx.needs_input_grad[0]:
             w = weight if weight.is_cuda else weight.detach().to(grad.device, non_blocking=True)
             if product == "mxfp4":
                 d4 = mx.quantize_mxfp4(grad, seed=seed, tensor_id=tensor_id, step=step)
-                gx = mx.mxfp4_matmul(d4, mx.quantize_mxfp4(w, transpose=True), dtype=ctx.x_dtype)
+                gx = mx.mxfp4_matmul(d4, mx.quantize_mxfp4(_rowed(w), transpose=True), dtype=ctx.x_dtype)
             else:
                 gx = grad @ w
         if codes is not None:
@@ -82,7 +92,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 class _GatedAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up, act):
-        h, g8, u8 = mx.gated_act(gate, up, act)
+        h, g8, u8 = mx.gated_act(_rowed(gate), _rowed(up), act)
         ctx.save_for_backward(g8.codes, g8.scales, u8.codes, u8.scales)
         ctx.shape, ctx.dtype, ctx.act = tuple(gate.shape), gate.dtype, act
         return h
@@ -93,7 +103,7 @@ class _GatedAct(torch.autograd.Function):
         gc, gs, uc, us = ctx.saved_tensors
         g8 = mx.MxTensor("mxint8", gc, gs, ctx.shape, ctx.dtype)
         u8 = mx.MxTensor("mxint8", uc, us, ctx.shape, ctx.dtype)
-        dgate, dup = mx.gated_act_backward(grad if grad.is_contiguous() else grad.contiguous(), g8, u8, ctx.act)
+        dgate, dup = mx.gated_act_backward(_rowed(grad), g8, u8, ctx.act)
         return dgate, dup, None
 
 

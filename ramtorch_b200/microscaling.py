@@ -70,29 +70,30 @@ class MxTensor:
     ``codes``: (rows, padded columns) int8 for ``"mxint8"``, (rows, padded columns / 2) uint8 for
     ``"mxfp4"``, two codes to a byte.  ``scales``: uint8, (rows, blocks padded to 4) for ``"mxint8"``;
     (row tiles of 128, block tiles of 4, 32, 4, 4) for ``"mxfp4"``, where scale (r, b) is at
-    ``[r // 128, b // 4, r % 32, r % 128 // 32, b % 4]``."""
+    ``[r // 128, b // 4, r % 32, r % 128 // 32, b % 4]``.  What fills up the last block of a row, and the
+    scales of rows and blocks that do not exist, are 0: products read them."""
 
     __slots__ = ("format", "codes", "scales", "shape", "dtype")
 
     def __init__(self, format: str, codes: torch.Tensor, scales: torch.Tensor, shape, dtype=torch.bfloat16):
         if format not in _FORMATS:
             raise ValueError(f"format must be 'mxint8' or 'mxfp4', not {format!r}")
-        shape = tuple(int(n) for n in shape)
-        if not shape or any(n < 0 for n in shape):
+        shape = tuple(shape)
+        if not shape or min(shape) < 0:
             raise ValueError("shape needs at least one dimension and no negative sizes")
         if dtype not in N.DTYPE_CODE:
             raise ValueError(f"unsupported dtype {dtype} (bf16, fp32, fp16 only)")
+        if not (codes.is_cuda and scales.is_cuda):
+            raise RuntimeError("codes and scales must be CUDA tensors: ramtorch_b200 has no CPU implementation")
         rows, cols = _split(shape)
         want_codes, want_scales = _layout(format, rows, cols)
-        for t, name, kind, want in ((codes, "codes", _CODES_DTYPE[format], want_codes),
-                                    (scales, "scales", torch.uint8, want_scales)):
-            if not t.is_cuda:
-                raise RuntimeError(f"{name} must be a CUDA tensor: ramtorch_b200 has no CPU implementation")
-            if t.dtype != kind or tuple(t.shape) != want or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous {kind} tensor of shape {want}")
-            if t.data_ptr() & 15:
-                raise ValueError(f"{name} must start on a 16-byte boundary")
-        if codes.device != scales.device:
+        if codes.dtype != _CODES_DTYPE[format] or codes.shape != want_codes or not codes.is_contiguous():
+            raise ValueError(f"codes must be a contiguous {_CODES_DTYPE[format]} tensor of shape {want_codes}")
+        if scales.dtype != torch.uint8 or scales.shape != want_scales or not scales.is_contiguous():
+            raise ValueError(f"scales must be a contiguous torch.uint8 tensor of shape {want_scales}")
+        if (codes.data_ptr() | scales.data_ptr()) & 15:
+            raise ValueError("codes and scales must start on 16-byte boundaries")
+        if codes.get_device() != scales.get_device():
             raise ValueError("codes and scales are on different devices")
         self.format, self.codes, self.scales, self.shape, self.dtype = format, codes, scales, shape, dtype
 
@@ -143,6 +144,7 @@ class MxTensor:
             if tuple(out.shape) != self.shape or out.device != self.codes.device:
                 raise ValueError("out has another shape or device")
             ld = _rows(out, "out")[2]
+            _apart(out, self)
         with _on(out.device):
             N.check(N.lib().rt_mx_dequantize(_FORMATS[self.format], self.codes.data_ptr(), self.scales.data_ptr(), rows, cols,
                                              out.data_ptr(), N.DTYPE_CODE[out.dtype], ld, N.stream_ptr(out.device.index)),
@@ -205,6 +207,24 @@ def _rows(x: torch.Tensor, name: str):
     return rows, cols, ld
 
 
+def _span(t):
+    """First byte of a tensor, and one past its last."""
+    if t.numel() == 0:
+        return 0, 0
+    first = t.data_ptr()
+    return first, first + (1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))) * t.element_size()
+
+
+def _apart(out, *inputs):
+    """The kernels read ahead of what they write: an output must not lie where an input does."""
+    a, b = _span(out)
+    for t in inputs:
+        for part in ((t.codes, t.scales) if isinstance(t, MxTensor) else (t,)):
+            c, d = _span(part)
+            if a < d and c < b:
+                raise ValueError("out overlaps an input")
+
+
 def _same_place(t, device, name):
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
@@ -265,6 +285,7 @@ def mxfp4_matmul(a: MxTensor, b: MxTensor, *, dtype=None, out: torch.Tensor | No
         ld = n
     else:
         ld = _check_out(out, shape, dtype, a.device)
+        _apart(out, a, b)
     with _on(a.device):
         N.check(N.lib().rt_mxfp4_matmul(a.codes.data_ptr(), a.scales.data_ptr(), b.codes.data_ptr(), b.scales.data_ptr(), m, n, k,
                                         out.data_ptr(), N.DTYPE_CODE[out.dtype], ld, N.stream_ptr(a.device.index)),
@@ -305,6 +326,7 @@ def weight_grad(grad_out: torch.Tensor, x8: MxTensor, *, dtype=None, out: torch.
         dtype, ld_out = _out_dtype(dtype or grad_out.dtype), k
     else:
         ld_out = _check_out(out, (n, k), dtype, grad_out.device)
+        _apart(out, grad_out, x8)
         dtype = out.dtype
     fast = _fast or _helper()
     if fast:
@@ -357,7 +379,8 @@ def gated_act(gate: torch.Tensor, up: torch.Tensor, act: str = "silu"):
 
 def gated_act_backward(grad_h: torch.Tensor, gate8: MxTensor, up8: MxTensor, act: str = "silu", *, out=None):
     """``(grad_gate, grad_up)`` of :func:`gated_act` from what it kept: ``grad_h * up8 * act'(gate8)`` and
-    ``grad_h * act(gate8)``.  ``out``: a pair of tensors to write to, e.g. the halves of one gradient."""
+    ``grad_h * act(gate8)``.  ``out``: a pair of tensors to write to, e.g. the halves of one gradient; as with
+    every ``out`` here, not where an input lies."""
     code = _act_code(act)
     rows, cols, ld = _rows(grad_h, "grad_h")
     for t, name in ((gate8, "gate8"), (up8, "up8")):
@@ -375,6 +398,13 @@ def gated_act_backward(grad_h: torch.Tensor, gate8: MxTensor, up8: MxTensor, act
     else:
         dgate, dup = out
         ld_gate, ld_up = (_check_out(t, grad_h.shape, grad_h.dtype, grad_h.device) for t in (dgate, dup))
+        for t in (dgate, dup):
+            _apart(t, grad_h, gate8, up8)
+        (a, b), (c, d) = _span(dgate), _span(dup)
+        if a < d and c < b:              # two tensors whose rows take turns, as the halves of one gradient do
+            off = abs(a - c) // dgate.element_size() % max(ld_gate, 1)
+            if ld_gate != ld_up or not cols <= off <= ld_gate - cols:
+                raise ValueError("the two outputs overlap")
     with _on(grad_h.device):
         N.check(N.lib().rt_mx_gated_act_backward(grad_h.data_ptr(), ld, N.DTYPE_CODE[grad_h.dtype], rows, cols, code,
                                                  gate8.codes.data_ptr(), gate8.scales.data_ptr(), up8.codes.data_ptr(),

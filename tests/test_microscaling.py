@@ -656,3 +656,44 @@ def test_both_host_sides_give_the_same(monkeypatch):
     monkeypatch.setattr(mx, "_fast", False)
     for s, t in zip(a, everything()):
         assert s.dtype == t.dtype and torch.equal(s, t)
+
+
+@gpu
+def test_outputs_may_not_lie_where_inputs_do():
+    x = torch.zeros(16, 64, device=DEV, dtype=torch.bfloat16)
+    q = mx.quantize_mxint8(x)
+    pool = torch.zeros(64, 256, device=DEV, dtype=torch.bfloat16)
+    g = pool[:16, :64]
+    for out in ((g, torch.zeros_like(x)), (torch.zeros_like(x), g), (x, x), (pool[20:36, :64], pool[21:37, :64]), (pool[20:36, :64], pool[20:36, 32:96])):
+        with pytest.raises(ValueError, match="overlap"):
+            mx.gated_act_backward(g, q, q, out=out)
+    mx.gated_act_backward(g, q, q, out=(pool[20:36, :64], pool[20:36, 64:128]))
+    mx.gated_act_backward(g, q, q, out=(pool[20:36, 128:192], pool[20:36, 64:128]))
+    mx.gated_act_backward(g, q, q, out=(pool[20:36, :64], pool[40:56, :64]))
+    with pytest.raises(ValueError, match="overlap"):
+        mx.weight_grad(pool[:16, :64], q, out=pool[:64, :64])
+    raw = q.codes.view(-1)[:16 * 64].view(torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        mx.MxTensor("mxint8", q.codes[:8], q.scales[:8], (8, 64)).dequantize(out=raw.view(8, 64))
+
+
+@gpu
+def test_layers_take_inputs_of_any_strides():
+    """Transposed and expanded inputs, weights and gradients, one vector, and an empty batch."""
+    torch.manual_seed(1)
+    w = torch.randn(48, 64, device=DEV).bfloat16()
+    xt = torch.randn(64, 33, device=DEV).bfloat16()
+    for product in (None, "mxfp4"):
+        for x in (xt.t(), xt.t()[:1].expand(5, 64), xt.t()[3], xt.t()[:0], xt.t().contiguous().view(3, 11, 64).transpose(0, 1)):
+            for weight in (w, w.t().contiguous().t()):
+                a, b = x.detach().requires_grad_(), weight.detach().requires_grad_()
+                y = ck.linear(a, b, product=product)
+                assert y.shape == x.shape[:-1] + (48,)
+                y.sum().backward()                      # an expanded gradient
+                plain = ck.linear(x.contiguous(), weight.contiguous(), product=product)
+                assert torch.equal(y.detach(), plain) or product is None
+                assert a.grad.shape == x.shape and b.grad.shape == w.shape
+                want = np.ones((48, 1)) * np64(mx.quantize_mxint8(x.reshape(-1, 64).contiguous()).dequantize(torch.float32)).sum(0)[None]
+                assert np.allclose(np64(b.grad), want, rtol=2.0 ** -7, atol=1e-3)
+    g, u = torch.randn(20, 30, device=DEV).t(), torch.randn(30, 20, device=DEV)
+    assert torch.equal(ck.gated_act(g, u), ck.gated_act(g.contiguous(), u))
