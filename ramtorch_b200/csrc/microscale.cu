@@ -2,8 +2,8 @@
 // MXFP4 for products.  Quantisation (nearest, and stochastic for MXFP4), its transposed form, the
 // way back, and the gated activation that keeps its inputs in MXINT8, with its backward pass.
 //
-// All of it is bound by memory: each value is read once and written once, 32 values share one
-// reduction of four lanes.  A thread handles UNITS of eight consecutive values of a row (16 bytes
+// Each value is read once and written once, 32 values share one reduction of four lanes; the traffic
+// bounds all of it but the stochastic rounding, which is bound by the integer pipe.  A thread handles UNITS of eight consecutive values of a row (16 bytes
 // of bf16 per access), the same unit of two or four consecutive rows: it works out once where that is,
 // and has all its loads under way before it uses the first.  Neighbouring threads have neighbouring
 // units of rows padded to whole blocks, so a block's four lanes are neighbours whatever the row length.
@@ -261,7 +261,9 @@ struct SrArgs {
 };
 
 // ------------------------------------------------------------------------------------- quantise
-// FMT 0: MXINT8, 1: MXFP4.
+// FMT 0: MXINT8, 1: MXFP4.  8192 x 11008 bf16: MXINT8 44 us (273 MB, 6.3 TB/s), MXFP4 41 us (228 MB, 5.5
+// TB/s, integer pipe 72 % busy).  Stochastic 88 us: the Philox rounds cost 29 of them and the rounding 18, on the same pipe.
+// Four rows to a thread (two: 50 us).
 constexpr int kRows = 4;   // rows to a thread
 
 template <int D, int FMT, bool SR, bool VEC>
@@ -304,7 +306,8 @@ mx_quantize_kernel(const Matrix x, const Grid g, uint8_t* __restrict__ codes, ui
 // rows, that is one or two whole blocks, so a block's maximum needs no exchange.  Eight
 // neighbouring columns x four blocks make a warp: an output row's four blocks (64 bytes) are
 // stored together.  The 32-byte pieces of a row are exchanged by the row's group of 32 (bits 3 and 4 of
-// the word index), which keeps those four lanes' reads in different banks.
+// the word index), which keeps those four lanes' reads in different banks.  8192 x 11008 bf16: 43 us, as
+// fast as along the rows; stochastic 76 us.
 constexpr int kTRows = 128, kTWords = 64;
 
 template <int D, bool SR, bool VEC>
@@ -373,6 +376,7 @@ mx_quantize_t_kernel(const Matrix x, const int64_t rows, const int cols, const u
 }
 
 // ----------------------------------------------------------------------------------- the way back
+// 8192 x 11008 to bf16: MXINT8 45 us (273 MB, 6.1 TB/s), MXFP4 41 us.
 template <int D, int FMT, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Grid g, const Matrix out) {
@@ -466,6 +470,8 @@ struct Kept {              // an MXINT8 matrix
   uint8_t* scales;
 };
 
+// 8192 x 11008 bf16, silu: forward 110 us (727 MB, 6.6 TB/s), backward 109 us; gelu 130 and 132, gelu_tanh 120 forward.
+// Two rows to a thread: one or four lose 15 % to too few loads under way or too few warps.
 constexpr int kPairs = 2;  // rows to a thread
 
 template <int D, int ACT, bool VEC>
