@@ -187,7 +187,7 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
 // slow index, so both are MN-major; a step takes 64 tokens.  The gradient's tile comes by TMA
 // ready for the tensor core; the codes' tile (8 KB) comes by TMA as bytes, the worker warps turn
 // it into bf16 (exact: a code times a power of two) in the swizzled layout.  fp32 and fp16
-// gradients arrive as up to three bf16 pieces that add up to them exactly; the pieces are further steps of the same sum.
+// gradients arrive as up to three bf16 pieces that add up to them; the pieces are further steps of the same sum.
 //
 // PAIR: two CTAs (ranks 2j and 2j + 1 of a cluster) make one tile of 256 features x BN, each with its own
 // 128 features and half of the gradient's columns, so that the gradient's tile is fetched and read half as
@@ -322,7 +322,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     int t = first % a.token_steps;
     for (int i = 0; i < count; ++i) {
       const int s = i % S::kStages;
-      if (!(ok = mbar_wait(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
+      if (!(ok = mbar_wait_warp(empty + 8 * s, ((i / S::kStages) & 1) ^ 1))) break;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int token = t * kTok + h * 32 + lane;
@@ -342,7 +342,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     const int mine = (warp - kFirstWorker) >> 2;
     for (int i = 0; i < count; ++i) {
       const int s = i % S::kStages, phase = (i / S::kStages) & 1;
-      if (!(ok = mbar_wait(full + 8 * s, phase))) break;      // every phase in turn: one that was left out could be taken for the next but one
+      if (!(ok = mbar_wait_warp(full + 8 * s, phase))) break;      // every phase in turn: one that was left out could be taken for the next but one
       if (i % kConvGroups != mine) continue;
       const uint8_t* in = smem + (codes - base) + s * S::kCodes + (w * 16 + low) * 128;
       const uint8_t* sc = smem + (scales - base) + s * S::kScales + (w * 16 + low) * 4;
@@ -380,7 +380,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
         else mbar_arrive(conv + 8 * s);
       }
     }
-    ok = mbar_wait(done, 0) && ok;
+    ok = mbar_wait_warp(done, 0) && ok;
     tc_fence_after();
   }
   __syncwarp();
@@ -392,8 +392,8 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
 }
 
 // A gradient that the tensor maps cannot take as it is (fp32, fp16, rows that do not start on 16-byte
-// boundaries) as bf16 planes whose sum it is: the leading 8 bits of each value's mantissa, the next 8,
-// the rest.  Cut, not rounded, so that nothing overflows; an infinity or a NaN is in the first plane alone.
+// boundaries) as bf16 planes whose sum it is (down to 2^-133, the last place of a bf16 number): the
+// leading 8 bits of each value's mantissa, the next 8, the rest.  Cut, not rounded, so that nothing overflows; an infinity or a NaN is in the first plane alone.
 // Eight values of a row to a thread, of two rows, planes of np = n rounded up to eight columns.
 template <int D, int P, bool VEC>
 __global__ void __launch_bounds__(256)
@@ -546,7 +546,7 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
       tc_commit<false>(done);
     }
   } else if (warp >= kFirstWorker) {
-    ok = mbar_wait(done, 0);
+    ok = mbar_wait_warp(done, 0);
     tc_fence_after();
   }
   __syncwarp();
@@ -677,7 +677,7 @@ mx_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_cons
     for (int t = blockIdx.x >> 1; t < tiles; t += pairs, ++n) {
       int m0, n0;
       place(t, m0, n0);
-      if (!(ok = mbar_wait(done, n & 1))) break;
+      if (!(ok = mbar_wait_warp(done, n & 1))) break;
       tc_fence_after();
       const int col = n0 + side * 128 + q * 32;
 #pragma unroll 1

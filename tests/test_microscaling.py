@@ -403,6 +403,24 @@ def test_weight_gradient_over_the_whole_exponent_range():
     assert torch.equal(mx.weight_grad(g.half(), q, dtype=torch.float32), q.dequantize(torch.float32))
 
 
+@gpu
+def test_weight_gradient_at_the_top_of_the_range():
+    """Scale bytes 253 and 254, next to ordinary blocks and to a block of zeros in the same warp's share."""
+    x = torch.randn(70, 200, device=DEV)
+    x[::3, :32] *= 2.0 ** 126 / 4
+    x[::3, 0] = 1.5 * 2.0 ** 126                         # fixes the scale byte at 253
+    x[1::3, 32:64] = torch.sign(x[1::3, 32:64]) * torch.finfo(torch.float32).max
+    x[5, 64:96] = 0
+    g = (torch.randn(70, 24, device=DEV) * 2.0 ** -60).bfloat16()
+    q = mx.quantize_mxint8(x)
+    assert set(q.scales[:, :2].unique().tolist()) & {253, 254} == {253, 254}
+    xv, gv = np64(q.dequantize(torch.float32)), np64(g)
+    assert np.isfinite(xv).all()
+    exact, mags = gv.T @ xv, np.abs(gv).T @ np.abs(xv)
+    got = np64(mx.weight_grad(g, q, dtype=torch.float32))
+    assert (np.abs(got - exact) <= sum_bound("f32", 70, exact, mags)).all()
+
+
 MATMUL = [(1, 1, 1), (1, 128, 128), (1, 300, 2080), (2, 64, 33), (8, 1001, 256), (17, 129, 64), (33, 40, 4096), (128, 128, 256), (130, 257, 520),
           (300, 100, 96), (257, 513, 1000), (64, 8, 11008)]
 
