@@ -614,13 +614,6 @@ def test_repeated_calls_give_the_same_bits():
 
 
 @gpu
-def test_no_wait_ran_out():
-    torch.cuda.synchronize()
-    count = ctypes.c_uint32(99)
-    assert N.lib().rt_mx_wait_faults(ctypes.byref(count)) == 0 and count.value == 0
-
-
-@gpu
 @pytest.mark.parametrize("tokens,n,k", [(64, 256, 256), (100, 300, 130), (700, 2100, 2500), (2000, 500, 4096), (320, 4000, 4500)])
 def test_weight_gradient_of_many_tiles(tokens, n, k):
     """Enough tiles, or tokens, for every tile shape and split; the last tiles of both sides are cut."""
@@ -715,3 +708,73 @@ def test_layers_take_inputs_of_any_strides():
                 assert np.allclose(np64(b.grad), want, rtol=2.0 ** -7, atol=1e-3)
     g, u = torch.randn(20, 30, device=DEV).t(), torch.randn(30, 20, device=DEV)
     assert torch.equal(ck.gated_act(g, u), ck.gated_act(g.contiguous(), u))
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements, and rows further apart than 2^31 bytes: the last rows are those of the same rows alone."""
+    rows, cols = 66000, 32800
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x.fill_(1.0)
+    tail = U.matrix(300, cols, "bf16", 21, 1.0, DEV)
+    x[-300:] = tail
+    q, t = mx.quantize_mxint8(x), mx.quantize_mxint8(tail)
+    assert torch.equal(q.codes[-300:], t.codes) and torch.equal(q.scales[-300:], t.scales) and (q.codes[:-300:997] == 64).all()
+    back = q.dequantize()
+    assert torch.equal(back[-300:], t.dequantize()) and (back[:-300:997] == 1).all()
+    del back
+    h, g8, u8 = mx.gated_act(x, x)
+    h2, g2, _ = mx.gated_act(tail, tail)
+    assert torch.equal(h[-300:], h2) and torch.equal(g8.codes[-300:], g2.codes)
+    dg, du = mx.gated_act_backward(x, g8, u8)
+    dg2, du2 = mx.gated_act_backward(tail, g2, g2)
+    assert torch.equal(dg[-300:], dg2) and torch.equal(du[-300:], du2)
+    del h, dg, du, g8, u8
+    p = mx.quantize_mxfp4(x)
+    assert torch.equal(p.dequantize(torch.bfloat16)[-300:], mx.quantize_mxfp4(tail).dequantize(torch.bfloat16))
+    p = mx.quantize_mxfp4(x, transpose=True)            # 32800 x 66000
+    cut = mx.quantize_mxfp4(x[:, -40:], transpose=True)
+    assert torch.equal(p.codes[-40:], cut.codes)
+    del p, x
+    # rows 2^31 bytes apart, at a misaligned start
+    far = torch.empty(4 * (1 << 30) + 4096, dtype=torch.bfloat16, device=DEV)
+    for ld in (1 << 30, (1 << 30) + 3):
+        v = far[1:].as_strided((4, 1000), (ld, 1))
+        v.copy_(U.matrix(4, 1000, "bf16", 22, 1.0, DEV))
+        w = v.contiguous()
+        assert torch.equal(mx.quantize_mxint8(v).codes, mx.quantize_mxint8(w).codes)
+        assert torch.equal(mx.quantize_mxfp4(v, transpose=True).codes, mx.quantize_mxfp4(w, transpose=True).codes)
+        g = torch.randn(4, 24, device=DEV).bfloat16()
+        out = mx.weight_grad(v, mx.quantize_mxint8(g))
+        assert torch.equal(out, mx.weight_grad(w, mx.quantize_mxint8(g)))
+        mx.quantize_mxint8(w).dequantize(out=v)
+        assert torch.equal(v, mx.quantize_mxint8(w).dequantize())
+
+
+@gpu
+def test_products_with_outputs_beyond_32_bits():
+    n, k = 48000, 46000
+    g = U.matrix(70, n, "bf16", 23, 1e-2, DEV, loud=False)
+    x = U.matrix(70, k, "bf16", 24, 1.0, DEV)
+    q = mx.quantize_mxint8(x)
+    dw = mx.weight_grad(g, q)
+    xv, gv = q.dequantize(torch.float32).double(), g.double()
+    for i, j in ((0, 0), (n - 300, k - 400), (n - 300, 0), (0, k - 400)):
+        a, b = gv[:, i:i + 300], xv[:, j:j + 400]
+        exact, mags = np64(a.T @ b), np64(a.T.abs() @ b.abs())
+        assert (np.abs(np64(dw[i:i + 300, j:j + 400]) - exact) <= sum_bound("bf16", 70, exact, mags)).all()
+    del dw
+    a4, b4 = mx.quantize_mxfp4(U.matrix(n, 96, "bf16", 25, 1.0, DEV)), mx.quantize_mxfp4(U.matrix(k, 96, "bf16", 26, 1.0, DEV))
+    y = mx.mxfp4_matmul(a4, b4)
+    av, bv = a4.dequantize(torch.float32).double(), b4.dequantize(torch.float32).double()
+    for i, j in ((0, 0), (n - 300, k - 400), (n - 300, 0), (0, k - 400)):
+        a, b = av[i:i + 300], bv[j:j + 400]
+        exact, mags = np64(a @ b.T), np64(a.abs() @ b.abs().T)
+        assert (np.abs(np64(y[i:i + 300, j:j + 400]) - exact) <= sum_bound("bf16", 96, exact, mags)).all()
+
+
+@gpu
+def test_no_wait_ran_out():
+    torch.cuda.synchronize()
+    count = ctypes.c_uint32(99)
+    assert N.lib().rt_mx_wait_faults(ctypes.byref(count)) == 0 and count.value == 0
