@@ -404,8 +404,8 @@ int rt_mx_gated_act_backward(const void* grad_h, int64_t ld_grad, int dtype, int
  * input).  Every product is exact (an fp32 gradient enters down to 2^-133), sums are fp32, one rounding to out's type.  accumulate != 0 adds to
  * out instead (the sum in fp32, rounded once).  grad_out: tokens x n, row stride ld_grad; out: n x k,
  * row stride ld_out.  workspace: device memory of at least rt_mx_weight_grad_workspace(...) bytes
- * for the same arguments (0 for bf16 gradients whose rows start on 16-byte boundaries), 16-byte
- * aligned, in use until the call's work on the stream is done.
+ * for the same arguments on the same device (often 0 for bf16 gradients whose rows start on 16-byte
+ * boundaries), 16-byte aligned, in use until the call's work on the stream is done.
  */
 int64_t rt_mx_weight_grad_workspace(const void* grad_out, int grad_dtype, int64_t ld_grad,
                                     int64_t tokens, int64_t n, int64_t k);

@@ -197,7 +197,7 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
 // What bounds it: at BN = 512 (all of tensor memory; a step's converted tile serves two products) the
 // tensor core, 486-502 us at 8192 x 4096 x 11008 = 1470-1520 TFLOP/s, 488 without the conversion; below that
 // the conversion, some 0.4 us a step (8192 codes; four integer operations to a pair, and the pipe
-// takes a warp in two clocks): 18 us at 2048 x 1024 x 4096 and at 16384 x 256 x 512.
+// takes a warp in two clocks): 18 us at 2048 x 1024 x 4096, 14 at 16384 x 256 x 512.
 constexpr int kTok = 64;
 
 template <int BN, bool PAIR>
@@ -216,6 +216,7 @@ struct WgradArgs {
   int tokens;
   int token_steps, pieces, splits;
   int k_tiles, n_tiles;                   // k_tiles: of 256 features with PAIR, else of 128
+  int64_t part;                           // 0, or bytes between the parts of a sum that another kernel joins (see join_parts_kernel)
   OutMatrix out;
 };
 
@@ -258,7 +259,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
   const int n0 = (group * 8 + in_group % width) * BN, k0 = (in_group / width * kCtas + side) * 128;
   const int64_t steps = (int64_t)a.token_steps * a.pieces;
   const int first = (int)(steps * split / a.splits), count = (int)(steps * (split + 1) / a.splits) - first;
-  const uint32_t leader = (uint32_t)(in_cluster & ~(kCtas - 1));
+  const uint32_t leader = PAIR ? cluster_rank() & ~1u : 0u;
 
   if (warp == 0 && elect_one()) {
     prefetch_map(&map_codes);
@@ -385,10 +386,33 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
   }
   __syncwarp();
   if (!ok) atomicAdd(&g_wait_faults, 1u);
-  finish_tile<BN, 4 * kConvGroups>(a.out, tmem, n0, k0, a.splits, side, kCtas, reinterpret_cast<float*>(smem), ok);
+  OutMatrix o = a.out;
+  if (a.part) o.p = static_cast<uint8_t*>(o.p) + split * a.part;
+  finish_tile<BN, 4 * kConvGroups>(o, tmem, n0, k0, a.part ? 1 : a.splits, side, kCtas, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
   if constexpr (PAIR) cluster_sync();        // the pair's products read both CTAs' memory, its barriers are in both
   if (warp == 2) tmem_free<PAIR>(tmem, kColumns);
+}
+
+// Few tiles and a long sum: more splits than a cluster has CTAs, each leaving its part of the output in
+// fp32, and this kernel adds them up in their order.  Four columns to a thread.  65536 x 256 x 512: 25 us
+// (in clusters of eight, which run 15 at a time, 54), 16384 x 256 x 512: 14 (18).
+__global__ void __launch_bounds__(256)
+join_parts_kernel(const float4* __restrict__ parts, const int64_t quads, const int splits, const FastDiv per_row, const OutMatrix o) {
+  const uint32_t q = blockIdx.x * 256 + threadIdx.x;
+  if (q >= quads) return;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const float4 v = __ldcs(parts + s * quads + q);
+    sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+  }
+  uint32_t r, c;
+  per_row.split(q, r, c);
+  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if ((int)c * 4 + j < o.cols) put_out(o, (int64_t)r * o.ld + c * 4 + j, v[j]);
 }
 
 // A gradient that the tensor maps cannot take as it is (fp32, fp16, rows that do not start on 16-byte
@@ -814,8 +838,43 @@ static int wgrad_at_once(int cluster) {
 template <int BN, bool PAIR>
 static int run_wgrad(const CUtensorMap& codes, const CUtensorMap& grad, const WgradArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> raised{0};
-  const int cluster = a.splits * (PAIR ? 2 : 1);
-  return launch_tc(mx_weight_grad_kernel<BN, PAIR>, raised, kWgradThreads, WgradSmem<BN, PAIR>::kBytes, (int64_t)a.k_tiles * a.n_tiles * cluster, cluster, st, codes, grad, a);
+  const int ctas = PAIR ? 2 : 1;
+  return launch_tc(mx_weight_grad_kernel<BN, PAIR>, raised, kWgradThreads, WgradSmem<BN, PAIR>::kBytes, (int64_t)a.k_tiles * a.n_tiles * a.splits * ctas,
+                   a.part ? ctas : a.splits * ctas, st, codes, grad, a);
+}
+
+// Tile and split of a weight gradient: the fewest nanoseconds, counted as rounds of what runs together times
+// (steps times what a step takes with this tile + start and output), and when split either the exchange in a cluster or the
+// parts' way through memory and the second launch; all measured.
+struct WgradPlan {
+  int bn, ctas, splits;
+  bool joined;                            // the parts are joined by join_parts_kernel
+  int64_t k_tiles, n_tiles;
+};
+static WgradPlan plan_wgrad(int64_t tokens, int64_t n, int64_t k, int pieces) {
+  const int64_t steps = (tokens + kTok - 1) / kTok * pieces;
+  struct Shape { int bn, ctas; double step, fixed; int (*at_once)(int); };
+  static const Shape shapes[] = {{512, 2, 560, 6000, wgrad_at_once<512, true>},
+                                 {256, 2, 400, 5000, wgrad_at_once<256, true>},
+                                 {128, 1, 380, 4500, wgrad_at_once<128, false>},
+                                 {64, 1, 360, 4000, wgrad_at_once<64, false>}};
+  WgradPlan p{};
+  double best = 1e300;
+  for (const Shape& c : shapes) {
+    const int64_t k_tiles = (k + 128 * c.ctas - 1) / (128 * c.ctas), n_tiles = (n + c.bn - 1) / c.bn, tiles = k_tiles * n_tiles;
+    for (int s = 1; s * c.ctas <= 8; ++s) {
+      if (s > steps || (s > 1 && c.bn > 256)) continue;      // a split tile has to fit into shared memory
+      const int at_once = c.at_once(s * c.ctas);
+      const double cost = (double)((tiles + at_once - 1) / at_once) * ((double)((steps + s - 1) / s) * c.step + c.fixed + (s > 1 ? 2000 : 0));
+      if (cost < best) { best = cost; p = {c.bn, c.ctas, s, false, k_tiles, n_tiles}; }
+    }
+    const int64_t s = std::min<int64_t>(c.at_once(c.ctas) / tiles, steps / 2);
+    if (s >= 2 && s * n * k <= ((int64_t)1 << 26)) {
+      const double cost = (double)((steps + s - 1) / s) * c.step + c.fixed + 3500 + (double)(s * n * k) * 8 / 4000;
+      if (cost < best) { best = cost; p = {c.bn, c.ctas, (int)s, true, k_tiles, n_tiles}; }
+    }
+  }
+  return p;
 }
 
 template <int BN>
@@ -845,8 +904,10 @@ extern "C" int64_t rt_mx_weight_grad_workspace(const void* grad_out, int grad_dt
   if (!dtype_ok(grad_dtype)) return fail(RT_E_DTYPE, "dtype code must be 0 (bf16), 1 (f32) or 2 (f16)");
   if (int rc = mx_check_shape(tokens, k)) return rc;
   if (int rc = mx_check_shape(tokens, n)) return rc;
-  if (tokens == 0 || n == 0 || k == 0 || taken_as_is(grad_out, grad_dtype, ld_grad)) return 0;
-  return pieces_of(grad_dtype) * tokens * pad_to(n, 8) * 2;
+  if (tokens == 0 || n == 0 || k == 0) return 0;
+  const int pieces = taken_as_is(grad_out, grad_dtype, ld_grad) ? 0 : pieces_of(grad_dtype);
+  const WgradPlan plan = plan_wgrad(tokens, n, k, std::max(1, pieces));
+  return pad_to(pieces * tokens * pad_to(n, 8) * 2, 16) + (plan.joined ? plan.splits * n * pad_to(k, 4) * 4 : 0);
 }
 
 extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, const void* codes, const void* scales,
@@ -874,7 +935,9 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   }
 
   const int64_t np = pad_to(n, 8), kp = pad_to(k, kMxBlock);
-  const int pieces = need ? pieces_of(grad_dtype) : 1;
+  const bool spread = !taken_as_is(grad_out, grad_dtype, ld_grad);
+  const int pieces = spread ? pieces_of(grad_dtype) : 1;
+  const WgradPlan plan = plan_wgrad(tokens, n, k, pieces);
   WgradArgs a{};
   a.scales = (const uint8_t*)scales;
   a.ld_scales = pad_to(kp / kMxBlock, 4);
@@ -883,27 +946,16 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
   a.pieces = pieces;
   a.out = {out, ld_out, (int)n, (int)k, out_dtype, accumulate != 0, aligned16(out, ld_out, dtype_size(out_dtype))};
 
-  // Tile and split: the fewest nanoseconds, counted as rounds of clusters that run together times
-  // (steps times what a step takes with this tile + start and output + the exchange when split), all measured.
-  const int64_t steps = (int64_t)a.token_steps * pieces;
-  struct Shape { int bn, ctas; double step, fixed; int (*at_once)(int); };
-  static const Shape shapes[] = {{512, 2, 560, 6000, wgrad_at_once<512, true>},
-                                 {256, 2, 400, 5000, wgrad_at_once<256, true>},
-                                 {128, 1, 380, 4500, wgrad_at_once<128, false>},
-                                 {64, 1, 360, 4000, wgrad_at_once<64, false>}};
-  const Shape* pick = nullptr;
-  double best = 1e300;
-  for (const Shape& c : shapes)
-    for (int s = 1; s * c.ctas <= 8; ++s) {
-      if (s > steps || (s > 1 && c.bn > 256)) continue;      // a split tile has to fit into shared memory
-      const int64_t tiles = (k + 128 * c.ctas - 1) / (128 * c.ctas) * ((n + c.bn - 1) / c.bn);
-      const int at_once = c.at_once(s * c.ctas);
-      const double cost = (double)((tiles + at_once - 1) / at_once) * ((double)((steps + s - 1) / s) * c.step + c.fixed + (s > 1 ? 2000 : 0));
-      if (cost < best) { best = cost; pick = &c; a.splits = s; }
-    }
-  a.k_tiles = (int)((k + 128 * pick->ctas - 1) / (128 * pick->ctas));
-  a.n_tiles = (int)((n + pick->bn - 1) / pick->bn);
-  if ((int64_t)a.k_tiles * a.n_tiles * a.splits * pick->ctas > 0x7FFFFFFFll) return fail(RT_E_SIZE, "n * k is too large");
+  const OutMatrix result = a.out;
+  a.splits = plan.splits;
+  a.k_tiles = (int)plan.k_tiles;
+  a.n_tiles = (int)plan.n_tiles;
+  if (plan.k_tiles * plan.n_tiles * a.splits * plan.ctas > 0x7FFFFFFFll) return fail(RT_E_SIZE, "n * k is too large");
+  const int64_t k4 = pad_to(k, 4);
+  if (plan.joined) {                        // the parts lie behind the planes
+    a.part = n * k4 * 4;
+    a.out = {(uint8_t*)workspace + (need - a.splits * a.part), k4, (int)n, (int)k4, RT_F32, 0, 1};
+  }
 
   CUtensorMap map_codes, map_grad;
   {
@@ -912,21 +964,26 @@ extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t l
     if (int rc = make_map(&map_codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   }
   {
-    const int64_t ld = need ? np : ld_grad;
-    const uint64_t dims[3] = {(uint64_t)n, (uint64_t)tokens, (uint64_t)pieces}, strides[2] = {(uint64_t)ld * 2, (uint64_t)(need ? tokens * np * 2 : ld * 2)};
+    const int64_t ld = spread ? np : ld_grad;
+    const uint64_t dims[3] = {(uint64_t)n, (uint64_t)tokens, (uint64_t)pieces}, strides[2] = {(uint64_t)ld * 2, (uint64_t)(spread ? tokens * np * 2 : ld * 2)};
     const uint32_t box[3] = {64, (uint32_t)kTok, 1};
-    if (int rc = make_map(&map_grad, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, need ? workspace : grad_out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    if (int rc = make_map(&map_grad, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, spread ? workspace : grad_out, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   }
-  if (need) {
+  if (spread) {
     if (grad_dtype == RT_F32) run_spread<RT_F32, 3>(grad_out, ld_grad, tokens, n, workspace, st);
     else if (grad_dtype == RT_F16) run_spread<RT_F16, 2>(grad_out, ld_grad, tokens, n, workspace, st);
     else run_spread<RT_BF16, 1>(grad_out, ld_grad, tokens, n, workspace, st);
     if (int rc = launched()) return rc;
   }
-  if (pick->bn == 512) return run_wgrad<512, true>(map_codes, map_grad, a, st);
-  if (pick->bn == 256) return run_wgrad<256, true>(map_codes, map_grad, a, st);
-  if (pick->bn == 128) return run_wgrad<128, false>(map_codes, map_grad, a, st);
-  return run_wgrad<64, false>(map_codes, map_grad, a, st);
+  if (int rc = plan.bn == 512   ? run_wgrad<512, true>(map_codes, map_grad, a, st)
+               : plan.bn == 256 ? run_wgrad<256, true>(map_codes, map_grad, a, st)
+               : plan.bn == 128 ? run_wgrad<128, false>(map_codes, map_grad, a, st)
+                                : run_wgrad<64, false>(map_codes, map_grad, a, st))
+    return rc;
+  if (!plan.joined) return 0;
+  const int64_t quads = n * (k4 / 4);
+  join_parts_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, st>>>((const float4*)a.out.p, quads, a.splits, FastDiv::of((uint32_t)(k4 / 4)), result);
+  return launched();
 }
 
 extern "C" int rt_mx_wait_faults(uint32_t* count) {

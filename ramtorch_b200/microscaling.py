@@ -334,11 +334,11 @@ def weight_grad(grad_out: torch.Tensor, x8: MxTensor, *, dtype=None, out: torch.
     if out is None:
         out = torch.empty((n, k), dtype=dtype, device=grad_out.device)
     L, code, g = N.lib(), N.DTYPE_CODE[grad_out.dtype], grad_out.data_ptr()
-    need = L.rt_mx_weight_grad_workspace(g, code, ld, tokens, n, k)
-    if need < 0:
-        N.check(int(need), "rt_mx_weight_grad_workspace")
-    space = torch.empty(need, dtype=torch.uint8, device=grad_out.device) if need else None
     with _on(grad_out.device):
+        need = L.rt_mx_weight_grad_workspace(g, code, ld, tokens, n, k)
+        if need < 0:
+            N.check(int(need), "rt_mx_weight_grad_workspace")
+        space = torch.empty(need, dtype=torch.uint8, device=grad_out.device) if need else None
         N.check(L.rt_mx_weight_grad(g, code, ld, x8.codes.data_ptr(), x8.scales.data_ptr(), tokens, n, k, out.data_ptr(),
                                     N.DTYPE_CODE[out.dtype], ld_out, accumulate, None if space is None else space.data_ptr(),
                                     need, N.stream_ptr(grad_out.device.index)), "rt_mx_weight_grad")

@@ -614,7 +614,7 @@ def test_repeated_calls_give_the_same_bits():
 
 
 @gpu
-@pytest.mark.parametrize("tokens,n,k", [(64, 256, 256), (100, 300, 130), (700, 2100, 2500), (2000, 500, 4096), (320, 4000, 4500)])
+@pytest.mark.parametrize("tokens,n,k", [(64, 256, 256), (100, 300, 130), (700, 2100, 2500), (2000, 500, 4096), (320, 4000, 4500), (9000, 130, 301), (20000, 8, 32), (6000, 250, 600)])
 def test_weight_gradient_of_many_tiles(tokens, n, k):
     """Enough tiles, or tokens, for every tile shape and split; the last tiles of both sides are cut."""
     x = U.matrix(tokens, k, "bf16", 15, 1.0, DEV)
