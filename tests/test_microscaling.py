@@ -404,6 +404,22 @@ def test_weight_gradient_over_the_whole_exponent_range():
 
 
 @gpu
+def test_weight_gradient_against_differences():
+    """The loss <grad, x8 @ w.T> is linear in w: along any direction v its difference quotient is <dw, v>, in 64 bits exactly."""
+    x, g = U.matrix(300, 136, "bf16", 31, 1.0, DEV), U.matrix(300, 72, "bf16", 32, 1e-2, DEV, loud=False)
+    q = mx.quantize_mxint8(x)
+    dw = mx.weight_grad(g, q, dtype=torch.float32).double()
+    x8, loss = q.dequantize(torch.float32).double(), lambda w: (g.double() * (x8 @ w.t())).sum()
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    w = torch.randn(72, 136, generator=gen, device=DEV, dtype=torch.float64)
+    for _ in range(4):
+        v = torch.randn(72, 136, generator=gen, device=DEV, dtype=torch.float64)
+        quotient = (loss(w + v) - loss(w - v)) / 2
+        bound = (v.abs() * (g.double().abs().t() @ x8.abs())).sum() * 302 * 2.0 ** -23
+        assert abs(quotient - (dw * v).sum()) <= bound
+
+
+@gpu
 def test_weight_gradient_at_the_top_of_the_range():
     """Scale bytes 253 and 254, next to ordinary blocks and to a block of zeros in the same warp's share."""
     x = torch.randn(70, 200, device=DEV)
@@ -508,6 +524,9 @@ def test_a_block_trains_like_its_plain_form(product):
     h = ck.gated_act(*proj.chunk(2, -1))
     y = ck.linear(h, w2, b2, tensor_id=1, **kw)
     gy = torch.randn_like(y)
+    # what is kept is 8 bits: the layers' inputs, and the two inputs of the activation
+    assert [t.dtype for t in proj.grad_fn.saved_tensors] == [torch.int8, torch.uint8, torch.bfloat16]
+    assert [t.dtype for t in h.grad_fn.saved_tensors] == [torch.int8, torch.uint8] * 2
     gx, g1, g2, gb, gproj, gh = torch.autograd.grad(y, (x, w1, w2, b2, proj, h), gy)
 
     def v64(a):
@@ -530,9 +549,6 @@ def test_a_block_trains_like_its_plain_form(product):
     a, b = values(gproj, **({"seed": 11, "step": 4} if product else {})), (values(w1, transpose=True).T if product else v64(w1))
     assert close(gx, a @ b, 2 * f, np.abs(a) @ np.abs(b))
     assert np.abs(np64(gb) - v64(gy).sum(0)).max() <= 2.0 ** -8 * np.abs(v64(gy).sum(0)).max() + 1e-4
-    # what is kept is 8 bits: the two inputs of the activation and the two layers' inputs
-    kept = [s for s in (proj.grad_fn, h.grad_fn, y.grad_fn)]
-    assert all(k is not None for k in kept)
 
 
 @gpu
