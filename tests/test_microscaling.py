@@ -620,6 +620,39 @@ def test_captured_and_replayed_and_on_another_stream():
 
 
 @gpu
+def test_a_training_step_captured_into_a_graph():
+    """Forward and backward of the layers inside one CUDA graph (leaves that no eager graph holds), replayed on new data."""
+    torch.manual_seed(5)
+    x = torch.randn(96, 128, device=DEV).bfloat16()
+    gy = torch.randn(96, 128, device=DEV).bfloat16()
+    shapes = [(2 * 160, 128), (128, 160)]
+    first = [torch.randn(*s, device=DEV).bfloat16() for s in shapes]
+
+    def step(ws):
+        h = ck.gated_act(*ck.linear(x, ws[0], product="mxfp4", seed=3, step=1).chunk(2, -1), "gelu_tanh")
+        y = ck.linear(h, ws[1], product="mxfp4", seed=3, tensor_id=1, step=1)
+        return torch.autograd.grad(y, ws, gy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step([w.clone().requires_grad_() for w in first])
+    torch.cuda.current_stream().wait_stream(side)
+    leaves = [w.clone().requires_grad_() for w in first]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step(leaves)
+    for _ in range(2):
+        x.copy_(torch.randn(96, 128, device=DEV))
+        gy.copy_(torch.randn(96, 128, device=DEV))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(grads, step([w.clone().requires_grad_() for w in first])):
+            assert torch.equal(a, b)
+
+
+@gpu
 def test_repeated_calls_give_the_same_bits():
     g, x = torch.randn(3000, 300, device=DEV).bfloat16(), torch.randn(3000, 200, device=DEV).bfloat16()
     q = mx.quantize_mxint8(x)
