@@ -1,6 +1,7 @@
 """ctypes binding of ``librt_b200.so`` (C ABI in ``include/rt_b200.h``).
 
-Nothing else in the package touches the shared library.  There is no CPU implementation
+Nothing else in the package touches the shared library, but for the optional ``_mxcall.so``, which
+``microscaling`` hands the addresses of the entry points found here.  There is no CPU implementation
 behind these calls: if the library has not been built the import fails with instructions.
 """
 from __future__ import annotations

@@ -267,7 +267,7 @@ struct SrArgs {
 constexpr int kRows = 4;   // rows to a thread
 
 template <int D, int FMT, bool SR, bool VEC>
-__global__ void __launch_bounds__(kMxThreads, SR || !VEC ? 1 : 6)
+__global__ void __launch_bounds__(kMxThreads, SR ? 1 : VEC ? 6 : D == RT_F32 ? 1 : 5)
 mx_quantize_kernel(const Matrix x, const Grid g, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, const SrArgs sr) {
   const Place<kRows> at(g);
   const int nb = g.upr.d >> 2;
@@ -471,11 +471,12 @@ struct Kept {              // an MXINT8 matrix
 };
 
 // 8192 x 11008 bf16, silu: forward 110 us (727 MB, 6.6 TB/s), backward 109 us; gelu 130 and 132, gelu_tanh 120 forward.
-// Two rows to a thread: one or four lose 15 % to too few loads under way or too few warps.
+// Two rows to a thread: one or four lose 15 % to too few loads under way or too few warps.  Rows off 16-byte
+// boundaries (8191 x 11007): 136 and 171 us, gelu 169 and 196.
 constexpr int kPairs = 2;  // rows to a thread
 
 template <int D, int ACT, bool VEC>
-__global__ void __launch_bounds__(kMxThreads, VEC && D != RT_F32 ? 5 : 1)
+__global__ void __launch_bounds__(kMxThreads, D != RT_F32 ? 5 : 1)
 mx_gated_kernel(const Matrix gate, const Matrix up, const Grid g, const Matrix h, const Kept kg, const Kept ku) {
   const Place<kPairs> at(g);
   const int nb = g.upr.d >> 2;
@@ -511,7 +512,7 @@ mx_gated_kernel(const Matrix gate, const Matrix up, const Grid g, const Matrix h
 }
 
 template <int D, int ACT, bool VEC>
-__global__ void __launch_bounds__(kMxThreads)
+__global__ void __launch_bounds__(kMxThreads, D == RT_F32 || VEC ? 1 : 5)
 mx_gated_backward_kernel(const Matrix grad, const Kept kg, const Kept ku, const Grid g, const Matrix dgate, const Matrix dup) {
   const uint32_t first = blockIdx.x * (kMxThreads * kPairs) + threadIdx.x;   // here a thread's units are a CTA's width apart
   const int stride = ((g.upr.d >> 2) + 3) & ~3;
