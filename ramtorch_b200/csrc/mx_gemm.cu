@@ -69,17 +69,33 @@ __device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col
 
 // 32 columns of the accumulator, from this warp's quarter of the lanes, as 32 output rows of 32 values:
 // through 2 KB of shared memory that the warp has to itself (fp32 in two halves), so that a lane stores 16
-// bytes of one row.  Straight from the registers, 64 bytes of one row to a warp, a column of a tile took
-// 17 ns, this way 8; TMA stores from shared memory were no faster.
+// bytes of one row.  The 16 bytes of a 64-byte row are exchanged by the row's bits 1 and 2, so that the
+// eight rows that a transposed store writes lie in different banks.  The instructions of this part bound tiles of
+// short sums: with a 16-bit store to each value 8 tokens x 4096 x 4096 took 21.5 us, with pairs rounded together and stored
+// transposed 18.6; MXFP4 8192 x 11008 x 4096 156 and 143.  Two squares at a time (19.3, 144) and TMA stores from shared memory were no faster.
 template <int D>
 __device__ __forceinline__ void put_room(const OutMatrix& o, int row, int col, const elem_t<D>* room) {
   constexpr int kLanes = D == RT_F32 ? 8 : 4, kPer = 16 / (int)sizeof(elem_t<D>), kRows = 32 / kLanes;   // lanes to a row, values to a lane, rows to a store
   const int lane = threadIdx.x & 31, c = col + lane % kLanes * kPer;
+  if (row + 4 * kRows <= o.rows && col + 32 <= o.cols) {
+    elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + (int64_t)(row + lane / kLanes) * o.ld + c;
+    const int64_t hop = kRows * o.ld;
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * kRows + lane / kLanes;
+      v[i] = *reinterpret_cast<const uint4*>(room + r * 32 + (D == RT_F32 ? lane % kLanes : lane % kLanes ^ (r >> 1 & 3)) * kPer);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(p + i * hop) = v[i];
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = i * kRows + lane / kLanes;
     if (row + r < o.rows && c < o.cols) {
-      const uint4 v = *reinterpret_cast<const uint4*>(room + r * 32 + lane % kLanes * kPer);
+      const int chunk = D == RT_F32 ? lane % kLanes : lane % kLanes ^ (r >> 1 & 3);
+      const uint4 v = *reinterpret_cast<const uint4*>(room + r * 32 + chunk * kPer);
       elem_t<D>* p = static_cast<elem_t<D>*>(o.p) + (int64_t)(row + r) * o.ld + c;
       if (c + kPer <= o.cols) *reinterpret_cast<uint4*>(p) = v;
       else {
@@ -92,22 +108,51 @@ __device__ __forceinline__ void put_room(const OutMatrix& o, int row, int col, c
   }
 }
 template <int D>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (D == RT_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <int D>
 __device__ __forceinline__ void put_square(const OutMatrix& o, uint32_t tmem, int row, int col, elem_t<D>* room) {
   const int lane = threadIdx.x & 31;
   uint32_t acc[2][16];
-  tmem_load16(tmem, acc[0]);
-  tmem_load16(tmem + 16, acc[1]);
-  tmem_wait(acc[0]);
-  tmem_wait(acc[1]);
+  if constexpr (D == RT_F32) {
+    tmem_load16(tmem, acc[0]);
+    tmem_load16(tmem + 16, acc[1]);
+    tmem_wait(acc[0]);
+    tmem_wait(acc[1]);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) room[((D == RT_F32 ? 0 : 16 * h) + j) * 32 + lane] = of_f32<D>(__uint_as_float(acc[h][j]));
-    if (D == RT_F32 || h == 1) {
+      for (int j = 0; j < 16; ++j) room[j * 32 + lane] = __uint_as_float(acc[h][j]);
       __syncwarp();
-      put_room<D>(o, D == RT_F32 ? row + 16 * h : row, col, room);
+      put_room<D>(o, row + 16 * h, col, room);
       __syncwarp();
     }
+  } else {
+    tmem_load_fragments(tmem, acc[0]);
+    tmem_load_fragments(tmem + (16u << 16), acc[1]);
+    tmem_wait(acc[0]);
+    tmem_wait(acc[1]);
+    const uint32_t to = smem_u32(room) + (lane & 7) * 64 + (((lane >> 3) ^ (lane >> 1 & 3)) << 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {            // eight columns, 32 lanes: four matrices
+      uint32_t w[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const uint32_t* p = acc[m >> 1] + 4 * i + 2 * (m & 1);
+        w[m] = pack2<D>(__uint_as_float(p[0]), __uint_as_float(p[1]));
+      }
+      store_transposed(to + i * 512, w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    put_room<D>(o, row, col, room);
+    __syncwarp();
   }
 }
 
@@ -390,7 +435,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
   if (a.part) o.p = static_cast<uint8_t*>(o.p) + split * a.part;
   finish_tile<BN, 4 * kConvGroups>(o, tmem, n0, k0, a.part ? 1 : a.splits, side, kCtas, reinterpret_cast<float*>(smem), ok);
   __syncthreads();
-  if constexpr (PAIR) cluster_sync();        // the pair's products read both CTAs' memory, its barriers are in both
+  if constexpr (PAIR) cluster_meet();        // the pair's products read both CTAs' memory, its barriers are in both
   if (warp == 2) tmem_free<PAIR>(tmem, kColumns);
 }
 

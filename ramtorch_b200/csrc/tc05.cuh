@@ -143,6 +143,21 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {     // names the 
                :
                : "memory");
 }
+// 16 lanes and 32 columns, as fragments of the matrix instructions: register 4 i + j of thread t holds
+// lane t / 4 + 8 (j / 2), column 8 i + 2 (t % 4) + j % 2.
+__device__ __forceinline__ void tmem_load_fragments(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+// Four 8 x 8 matrices of 16-bit values, transposed, to shared memory: lane 8 m + r gives the address of
+// 16 bytes for column r of matrix m.
+__device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 
 // ------------------------------------------------------------------------------------ descriptors
 // A tile in shared memory, 128-byte swizzle.  Rows of 128 bytes, eight to a swizzle atom (1024
@@ -208,6 +223,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same for control alone: nothing that was written before has to be seen after it, so that no store is waited for.
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // Arrives at the barrier that CTA `rank` of the cluster has at the place of `bar`.  A release at cluster
 // scope would wait for all of this thread's memory traffic (0.3 us); what the arrival announces are
