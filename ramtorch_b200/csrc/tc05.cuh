@@ -224,7 +224,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// The same for control alone: nothing that was written before has to be seen after it, so that no store is waited for.
+// As cluster_sync, for control alone: nothing that was written before has to be seen after it, so that no store is waited for.
 __device__ __forceinline__ void cluster_meet() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }

@@ -374,6 +374,29 @@ def test_weight_gradient(tokens, n, k, kind):
 
 
 @gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("tokens,n,k", [(1, 1, 1), (5, 33, 8), (17, 257, 129), (64, 600, 135), (300, 40, 1000), (77, 1030, 4103), (700, 64, 65)])
+def test_weight_gradient_added_to_aligned_rows(tokens, n, k, kind):
+    """Rows on 16-byte boundaries, ends inside and at the end of 16 bytes; what lies around stays."""
+    q = mx.quantize_mxint8(U.matrix(tokens, k, "bf16", 15, 1.0, DEV))
+    g = U.matrix(tokens, n, "bf16", 16, 1e-2, DEV, loud=False)
+    held = U.matrix(n, k, kind, 17, 1.0, DEV)
+    buf = torch.full((n + 2, (k + 15) // 8 * 8), 7.0, dtype=U.TORCH[kind], device=DEV)
+    out = buf[1:1 + n, :k]
+    out.copy_(held)
+    mx.weight_grad(g, q, out=out, accumulate=True)
+    xv, gv, hv = np64(q.dequantize(torch.float32)), np64(g), np64(held)
+    exact, mags = gv.T @ xv + hv, np.abs(gv).T @ np.abs(xv) + np.abs(hv)
+    assert (np.abs(np64(out) - exact) <= sum_bound(kind, tokens + 1, exact, mags)).all()
+    assert (buf[0] == 7).all() and (buf[-1] == 7).all() and (buf[:, k:] == 7).all()
+    again = torch.empty_like(held)
+    again.copy_(held)
+    mx.weight_grad(g, q, out=again, accumulate=True)      # the same sum wherever it lies
+    if k % 8 == 0:
+        assert torch.equal(again, out)
+
+
+@gpu
 def test_weight_gradient_of_nothing_and_of_nan():
     g, x = torch.ones(0, 24, device=DEV, dtype=torch.bfloat16), torch.ones(0, 40, device=DEV, dtype=torch.bfloat16)
     q = mx.quantize_mxint8(x)
