@@ -949,8 +949,9 @@ static int run_wgrad(const CUtensorMap& codes, const CUtensorMap& grad, const Wg
 }
 
 // Tile and split of a weight gradient: the fewest nanoseconds, counted as rounds of what runs together times
-// (steps times what a step takes with this tile + start and output), and when split either the exchange in a cluster or the
-// parts' way through memory and the second launch; all measured.
+// (steps times what a step takes with this tile + start and output), and when split either the exchange in a cluster (1.2 us
+// and 33 ns to a column of a CTA's share) or the parts' way through memory and the second launch; all measured
+// (1024 x 1024 x 1024: 9.8 us unsplit in 128 x 64, 11.9 in 256 x 256 with the sum in three).
 struct WgradPlan {
   int bn, ctas, splits;
   bool joined;                            // the parts are joined by join_parts_kernel
@@ -970,12 +971,12 @@ static WgradPlan plan_wgrad(int64_t tokens, int64_t n, int64_t k, int pieces) {
     for (int s = 1; s * c.ctas <= 8; ++s) {
       if (s > steps || (s > 1 && c.bn > 256)) continue;      // a split tile has to fit into shared memory
       const int at_once = c.at_once(s * c.ctas);
-      const double cost = (double)((tiles + at_once - 1) / at_once) * ((double)((steps + s - 1) / s) * c.step + c.fixed + (s > 1 ? 2000 : 0));
+      const double cost = (double)((tiles + at_once - 1) / at_once) * ((double)((steps + s - 1) / s) * c.step + c.fixed + (s > 1 ? 1200 + 33.0 * c.bn / s : 0));
       if (cost < best) { best = cost; p = {c.bn, c.ctas, s, false, k_tiles, n_tiles}; }
     }
     const int64_t s = std::min<int64_t>(c.at_once(c.ctas) / tiles, steps / 2);
     if (s >= 2 && s * n * k <= ((int64_t)1 << 26)) {
-      const double cost = (double)((steps + s - 1) / s) * c.step + c.fixed + 3500 + (double)(s * n * k) * 8 / 4000;
+      const double cost = (double)((steps + s - 1) / s) * c.step + c.fixed + 3500 + (double)(s * n * k) * 8 / 8000;     // written and read in L2
       if (cost < best) { best = cost; p = {c.bn, c.ctas, (int)s, true, k_tiles, n_tiles}; }
     }
   }
@@ -1124,7 +1125,7 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
 
   // Tile and split, by the microseconds that were measured for each: a start, then rounds of what runs
   // together.  Unsplit tiles run two to an SM and slow each other down; clusters run one CTA to an SM.
-  // (8192 x 11008 x 4096: 208 us in 128 x 128 tiles, 154 in pairs; 2048 x 4096 x 4096: 24 and 27; 1 x 4096 x 4096:
+  // (4096 x 4096 x 4096: 45 us in 128 x 128 tiles, 38 in pairs; 2048 x 4096 x 4096: 23 and 25; 1 x 4096 x 4096:
   // 8.9 unsplit, 6.4 in four.)
   const int64_t n_tiles = (n + 127) / 128;
   const int width = m <= 32 ? 32 : m <= 64 ? 64 : 128;      // rows of a to a tile: narrow ones only for a single tile
@@ -1133,15 +1134,16 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
   double best = 1e300;
   for (int s = 1; s <= 8 && s <= a.steps; ++s) {
     const int at_once = s == 1 ? 2 * kSms : width == 128 ? fp4_at_once<128>(s) : width == 64 ? fp4_at_once<64>(s) : fp4_at_once<32>(s);
-    const double step = s > 1 ? 0.34 : 0.34 + 0.26 * std::min(1.0, std::max(0.0, (double)(tiles - kSms) / kSms));
-    const double cost = 4.0 + (s > 1 ? 1.5 : 0) + (double)((tiles + at_once - 1) / at_once) * ((double)((a.steps + s - 1) / s) * step + (s > 1 ? 1.0 : 1.5)) - 1.5;
+    const double both = s > 1 ? 0 : std::min(1.0, std::max(0.0, (double)(tiles - kSms) / kSms));     // how far tiles share an SM
+    const double round = (double)((a.steps + s - 1) / s) * (0.34 + 0.15 * both) + (s > 1 ? 3.0 : 1.2 + 1.5 * both);
+    const double cost = (s > 1 ? 2.0 : 2.5) + (double)((tiles + at_once - 1) / at_once) * round;
     if (cost < best) { best = cost; splits = s; }
   }
   const int64_t pair_tiles = (n + 255) / 256 * ((m + 383) / 384);
   if (pair_tiles > 0x3FFFFFFFll) return fail(RT_E_SIZE, "m * n is too large");
   if (m > 128) {
     const int at_once = fp4_pairs_at_once();
-    if (3.5 + (double)((pair_tiles + at_once - 1) / at_once) * (a.steps * 0.58 + 2.2) < best) bm = 384;
+    if (3.5 + (double)((pair_tiles + at_once - 1) / at_once) * (a.steps * 0.5 + 3.0) < best) bm = 384;
   }
   a.splits = splits;
   a.n_tiles = (int)n_tiles;
