@@ -300,7 +300,7 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
 // products; both CTAs' workers arrive at its barrier.
 //
 // What bounds it: at BN = 512 (all of tensor memory; a step's converted tile serves two products) the
-// tensor core, 486-502 us at 8192 x 4096 x 11008 = 1470-1520 TFLOP/s, 488 without the conversion; below that
+// tensor core, 472-481 us at 8192 x 4096 x 11008 = 1540-1560 TFLOP/s (taking out the conversion changed nothing); below that
 // the conversion, some 0.4 us a step (8192 codes; four integer operations to a pair, and the pipe
 // takes a warp in two clocks): 18 us at 2048 x 1024 x 4096, 14 at 16384 x 256 x 512.
 constexpr int kTok = 64;
@@ -690,8 +690,8 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
 // the small tiles above is the way from L2: 34 KB per CTA for 256 clocks of products at 128 x 128,
 // here 44 KB for 768.  384 columns of sums and four stages of scales (8 columns of b's, 24 of a's) fill
 // tensor memory, so a tile's output is not overlapped with the next one's products, but its loads are.
-// 8192 x 11008 x 4096: 154 us (4.8 PFLOP/s), 8192 x 8192 x 8192: 199 us (5.5); a step takes 0.5 us, of which the
-// products are 0.4, and a tile's start and output 2.
+// 8192 x 11008 x 4096: 143 us (5.2 PFLOP/s), 8192 x 8192 x 8192: 188 us (5.8); a step takes 0.5 us, of which the
+// products are 0.4, and a tile's start and output 3.
 // Every CTA needs the scales of all 384 rows of a.  Both CTAs' loads report to the first one's barrier (told
 // by a warp of the second instead, a step took 550 ns); the first issues all copies and products.
 struct PairSmem {
