@@ -372,7 +372,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(full + 8 * s, 1 + 32);       // the loads, and warp 3's lanes
       mbar_init(empty + 8 * s, 1);
-      mbar_init(conv + 8 * s, 4 * kCtas);    // the four warps of a step, of both CTAs
+      mbar_init(conv + 8 * s, 4 * kConvGroups * kCtas);    // all converting warps, of both CTAs
     }
     mbar_init(done, 1);
     fence_barrier_init();
@@ -448,8 +448,16 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
     const int mine = (warp - kFirstWorker) >> 2;
     for (int i = 0; i < count; ++i) {
       const int s = i % S::kStages, phase = (i / S::kStages) & 1;
-      if (!(ok = mbar_wait_warp(full + 8 * s, phase))) break;      // every phase in turn: one that was left out could be taken for the next but one
-      if (i % kConvGroups != mine) continue;
+      // Every phase in turn: one that was left out could be taken for the next but one.  The group whose step it
+      // is not says so as well, at once: the stage is not filled anew before both groups have seen this phase, so none can pass unseen.
+      if (!(ok = mbar_wait_warp(full + 8 * s, phase))) break;
+      if (i % kConvGroups != mine) {
+        if (lane == 0) {
+          if constexpr (PAIR) mbar_arrive_at(conv + 8 * s, leader);
+          else mbar_arrive(conv + 8 * s);
+        }
+        continue;
+      }
       const uint8_t* in = smem + (codes - base) + s * S::kCodes + (w * 16 + low) * 128;
       const uint8_t* sc = smem + (scales - base) + s * S::kScales + (w * 16 + low) * 4;
       uint8_t* out = smem + (tile_a - base) + s * S::kA + (w * 16 + low) * 128;
