@@ -5,7 +5,7 @@
     y = linear(x, weight, product="mxfp4", seed=7, step=t)   # 4-bit products forward and for grad_x
 
 Both take part in autograd like their torch counterparts.  The weight gradient comes straight from
-the 8-bit codes (``microscaling.weight_grad``); for a CPU-resident weight it is added to
+the 8-bit codes (``microscaling.weight_grad``); for a CPU-resident ``is_ramtorch`` parameter it is added to
 ``weight.rt_device_grad`` in HBM, where ``AdamW.step`` takes it (``helpers.accumulate_weight_grad``).
 """
 from __future__ import annotations
@@ -23,6 +23,12 @@ def _rowed(t: torch.Tensor) -> torch.Tensor:
         return t
     except ValueError:
         return t.contiguous()
+
+
+def _handed_over(weight: torch.Tensor) -> bool:
+    """Whether a weight's gradient stays in HBM as ``rt_device_grad``: only where the optimizer will look for it, on a
+    flagged host parameter itself.  What was made of a parameter (a cast, a slice) has to pass its gradient on through autograd."""
+    return not weight.is_cuda and weight.is_leaf and getattr(weight, "is_ramtorch", False)
 
 
 class _Linear(torch.autograd.Function):
@@ -58,10 +64,10 @@ class _Linear(torch.autograd.Function):
                 gx = grad @ w
         if codes is not None:
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
-            if weight.is_cuda:
-                gw = mx.weight_grad(grad, x8, dtype=weight.dtype)
-            else:
+            if _handed_over(weight):
                 helpers.accumulate_weight_grad(weight, grad, x8)
+            else:
+                gw = mx.weight_grad(grad, x8, dtype=weight.dtype).to(weight.device)
         if ctx.bias_like is not None and ctx.needs_input_grad[2]:
             gb = grad.reshape(-1, grad.shape[-1]).sum(0, dtype=torch.float32).to(**ctx.bias_like)
         return gx, gw, gb, None, None, None, None
@@ -76,8 +82,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``seed`` is given (Philox draws ``(seed, tensor_id, step)``: pass another ``tensor_id`` for each layer
     and count ``step``), else to nearest.  The weight gradient always takes the gradient unrounded.
 
-    A weight in host memory (``is_ramtorch`` parameters) is copied to x's device for the product, and
-    its gradient stays there as ``weight.rt_device_grad``."""
+    A weight in host memory is copied to x's device for the product.  The gradient of an ``is_ramtorch``
+    parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the
+    flag, a cast or a slice of a parameter) goes to host memory through autograd."""
     if product not in (None, "mxfp4"):
         raise ValueError(f"product must be None or 'mxfp4', not {product!r}")
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:

@@ -1,0 +1,71 @@
+"""The layers of ramtorch_b200.checkpointing as training programs call them: host weights of every kind, recomputation,
+ZeRO-2 hooks, automatic mixed precision, and what they refuse."""
+import numpy as np
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from ramtorch_b200 import checkpointing as ck
+from ramtorch_b200 import helpers
+from ramtorch_b200 import microscaling as mx
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+T, N, K = 33, 40, 72
+
+
+def np64(t):
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def randn(*shape, seed, dtype=torch.bfloat16, device=DEV):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).to(device=device, dtype=dtype)
+
+
+def held(p):
+    return p.__dict__.get(helpers.DEVICE_GRAD_ATTR)
+
+
+def host_parameter(seed=1, flagged=True, dtype=torch.bfloat16, shape=(N, K)):
+    p = torch.nn.Parameter(randn(*shape, seed=seed, dtype=dtype, device="cpu").mul_(0.1).pin_memory())
+    if flagged:
+        p.is_ramtorch = True
+    return p
+
+
+def dw_of(x, g, dtype=torch.bfloat16):
+    return mx.weight_grad(g, mx.quantize_mxint8(x), dtype=dtype)
+
+
+# ------------------------------------------------------------------------------------- host weights
+@gpu
+@pytest.mark.parametrize("flagged", [False, True])
+def test_a_cast_or_a_part_of_a_host_parameter_gets_its_gradient(flagged):
+    """What autograd made of a parameter hands the gradient on to the parameter."""
+    x, g = randn(T, K, seed=2), randn(T, N, seed=3)
+    master = host_parameter(flagged=flagged, dtype=torch.float32)
+    ck.linear(x, master.bfloat16()).backward(g)
+    want = dw_of(x, g)
+    assert held(master) is None and torch.equal(master.grad, want.float().cpu())
+    both = host_parameter(flagged=flagged, shape=(2 * N, K))
+    part = both[N:]
+    part.is_ramtorch = True                  # a flag on what is no leaf changes nothing
+    ck.linear(x, part).backward(g)
+    assert held(both) is None and held(part) is None
+    assert torch.equal(both.grad[N:], want.cpu()) and (both.grad[:N] == 0).all()
+
+
+@gpu
+def test_a_host_leaf_without_the_flag_gets_an_ordinary_gradient():
+    w = host_parameter(flagged=False)
+    xs, gs = [randn(T, K, seed=s) for s in (2, 3)], [randn(T, N, seed=s) for s in (4, 5)]
+    ck.linear(xs[0], w).backward(gs[0])
+    assert held(w) is None and torch.equal(w.grad, dw_of(xs[0], gs[0]).cpu())
+    ck.linear(xs[1], w).backward(gs[1])
+    assert torch.equal(w.grad, dw_of(xs[0], gs[0]).cpu() + dw_of(xs[1], gs[1]).cpu())
+    got, = torch.autograd.grad(ck.linear(xs[0], w), (w,), gs[0])
+    assert torch.equal(got, dw_of(xs[0], gs[0]).cpu())
+    before = w.detach().clone()
+    torch.optim.SGD([w], lr=1.0).step()
+    assert torch.equal(w.detach(), before - w.grad)
