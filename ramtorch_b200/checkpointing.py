@@ -44,6 +44,8 @@ class _Linear(torch.autograd.Function):
             y = y + bias.to(x.device)
         keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(*((keep.codes, keep.scales) if keep is not None else (None, None)), weight)
+        # the parameter itself: what is saved comes back as another tensor after recomputation or through saved-tensor hooks
+        ctx.handed_over = weight if _handed_over(weight) else None
         ctx.x_shape, ctx.x_dtype, ctx.args = tuple(x.shape), x.dtype, (product, seed, tensor_id, step)
         ctx.bias_like = None if bias is None else {"dtype": bias.dtype, "device": bias.device}
         return y
@@ -64,8 +66,8 @@ class _Linear(torch.autograd.Function):
                 gx = grad @ w
         if codes is not None:
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
-            if _handed_over(weight):
-                helpers.accumulate_weight_grad(weight, grad, x8)
+            if ctx.handed_over is not None:
+                helpers.accumulate_weight_grad(ctx.handed_over, grad, x8)
             else:
                 gw = mx.weight_grad(grad, x8, dtype=weight.dtype).to(weight.device)
         if ctx.bias_like is not None and ctx.needs_input_grad[2]:
@@ -84,7 +86,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
 
     A weight in host memory is copied to x's device for the product.  The gradient of an ``is_ramtorch``
     parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the
-    flag, a cast or a slice of a parameter) goes to host memory through autograd."""
+    flag, a cast or a slice of a parameter) goes to host memory through autograd.  ``AdamW.step`` takes
+    ``rt_device_grad`` in place of ``grad``: a flagged parameter should get all of its gradient from one of the two."""
     if product not in (None, "mxfp4"):
         raise ValueError(f"product must be None or 'mxfp4', not {product!r}")
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:

@@ -69,3 +69,19 @@ def test_a_host_leaf_without_the_flag_gets_an_ordinary_gradient():
     before = w.detach().clone()
     torch.optim.SGD([w], lr=1.0).step()
     assert torch.equal(w.detach(), before - w.grad)
+
+
+@gpu
+@pytest.mark.parametrize("way", ["recomputed", "recomputed, reentrant", "saved on the host"])
+def test_a_host_parameter_keeps_its_gradient_when_saved_tensors_are_packed(way):
+    """Recomputation and saved-tensor hooks hand other tensors to the backward pass than the forward saved."""
+    w, x, g = host_parameter(), randn(T, K, seed=2).requires_grad_(), randn(T, N, seed=3)
+    if way == "saved on the host":
+        with torch.autograd.graph.save_on_cpu(pin_memory=True):
+            y = ck.linear(x, w)
+    else:
+        y = checkpoint(lambda a: ck.linear(a, w), x, use_reentrant="reentrant" in way)
+    y.backward(g)
+    assert torch.equal(held(w), dw_of(x, g)) and w.grad is None
+    plain, = torch.autograd.grad(ck.linear(x, w), (x,), g)
+    assert torch.equal(x.grad, plain)
