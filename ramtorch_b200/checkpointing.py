@@ -25,10 +25,10 @@ def _rowed(t: torch.Tensor) -> torch.Tensor:
         return t.contiguous()
 
 
-def _handed_over(weight: torch.Tensor) -> bool:
-    """Whether a weight's gradient stays in HBM as ``rt_device_grad``: only where the optimizer will look for it, on a
-    flagged host parameter itself.  What was made of a parameter (a cast, a slice) has to pass its gradient on through autograd."""
-    return not weight.is_cuda and weight.is_leaf and getattr(weight, "is_ramtorch", False)
+def _flagged(p: torch.Tensor | None):
+    """`p` if it is an ``is_ramtorch`` parameter itself, else None.  What was made of a parameter (a cast, a slice) has to
+    pass its gradient on through autograd."""
+    return p if p is not None and p.is_leaf and getattr(p, "is_ramtorch", False) else None
 
 
 class _Linear(torch.autograd.Function):
@@ -44,8 +44,8 @@ class _Linear(torch.autograd.Function):
             y = y + bias.to(x.device)
         keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(*((keep.codes, keep.scales) if keep is not None else (None, None)), weight)
-        # the parameter itself: what is saved comes back as another tensor after recomputation or through saved-tensor hooks
-        ctx.handed_over = weight if _handed_over(weight) else None
+        # the parameters themselves: what is saved comes back as another tensor after recomputation or through saved-tensor hooks
+        ctx.flagged = _flagged(weight), _flagged(bias)
         ctx.x_shape, ctx.x_dtype, ctx.args = tuple(x.shape), x.dtype, (product, seed, tensor_id, step)
         ctx.bias_like = None if bias is None else {"dtype": bias.dtype, "device": bias.device}
         return y
@@ -66,12 +66,14 @@ class _Linear(torch.autograd.Function):
                 gx = grad @ w
         if codes is not None:
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
-            if ctx.handed_over is not None:
-                helpers.accumulate_weight_grad(ctx.handed_over, grad, x8)
+            if ctx.flagged[0] is not None and not weight.is_cuda:
+                helpers.accumulate_weight_grad(ctx.flagged[0], grad, x8)
             else:
-                gw = mx.weight_grad(grad, x8, dtype=weight.dtype).to(weight.device)
+                gw = mx.weight_grad(grad, x8, dtype=weight.dtype)
+                gw = helpers.invoke_ramtorch_hooks(ctx.flagged[0], gw).to(weight.device)
         if ctx.bias_like is not None and ctx.needs_input_grad[2]:
-            gb = grad.reshape(-1, grad.shape[-1]).sum(0, dtype=torch.float32).to(**ctx.bias_like)
+            gb = grad.reshape(-1, grad.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_like["dtype"])
+            gb = helpers.invoke_ramtorch_hooks(ctx.flagged[1], gb).to(ctx.bias_like["device"])
         return gx, gw, gb, None, None, None, None
 
 
@@ -87,7 +89,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     A weight in host memory is copied to x's device for the product.  The gradient of an ``is_ramtorch``
     parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the
     flag, a cast or a slice of a parameter) goes to host memory through autograd.  ``AdamW.step`` takes
-    ``rt_device_grad`` in place of ``grad``: a flagged parameter should get all of its gradient from one of the two."""
+    ``rt_device_grad`` in place of ``grad``: a flagged parameter should get all of its gradient from one of the two.
+    ZeRO-2 hooks of flagged parameters see the fresh gradient, of a weight and of a bias, before it is added anywhere."""
     if product not in (None, "mxfp4"):
         raise ValueError(f"product must be None or 'mxfp4', not {product!r}")
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:

@@ -85,3 +85,25 @@ def test_a_host_parameter_keeps_its_gradient_when_saved_tensors_are_packed(way):
     assert torch.equal(held(w), dw_of(x, g)) and w.grad is None
     plain, = torch.autograd.grad(ck.linear(x, w), (x,), g)
     assert torch.equal(x.grad, plain)
+
+
+# -------------------------------------------------------------------------------------- ZeRO-2 hooks
+@gpu
+def test_zero2_hooks_see_the_gradient_of_a_bias_and_of_a_weight_in_hbm():
+    """The hook dict of a flagged parameter runs on every fresh gradient: autograd itself knows nothing of it."""
+    w, b = host_parameter(), torch.nn.Parameter(randn(N, seed=9, device="cpu"))
+    b.is_ramtorch = True
+    seen = []
+    helpers.register_ramtorch_hook(b, lambda t: seen.append(t.clone()) or t * 4, helpers.ZERO2_HOOK_NAME)
+    x, gs = randn(T, K, seed=2), [randn(T, N, seed=s) for s in (4, 5)]
+    for g in gs:
+        ck.linear(x, w, b).backward(g)
+    assert [t.is_cuda for t in seen] == [True, True]
+    for s, g in zip(seen, gs):
+        assert torch.equal(s, g.sum(0, dtype=torch.float32).bfloat16())
+    assert torch.equal(b.grad, (seen[0] * 4).cpu() + (seen[1] * 4).cpu())
+    v = torch.nn.Parameter(randn(N, K, seed=1))
+    v.is_ramtorch = True
+    helpers.register_ramtorch_hook(v, lambda t: t * 2, helpers.ZERO2_HOOK_NAME)
+    ck.linear(x, v).backward(gs[0])
+    assert torch.equal(v.grad, dw_of(x, gs[0]) * 2)
