@@ -97,6 +97,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     if x.dtype != weight.dtype:
         raise ValueError(f"x is {x.dtype} and weight {weight.dtype}")
+    if bias is not None and (bias.dtype != x.dtype or bias.shape != weight.shape[:1]):
+        raise ValueError(f"bias must be {x.dtype} of shape {tuple(weight.shape[:1])}, not {bias.dtype} {tuple(bias.shape)}")
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor: ramtorch_b200 has no CPU implementation")
     return _Linear.apply(x, weight, bias, product, seed, tensor_id, step)

@@ -107,3 +107,13 @@ def test_zero2_hooks_see_the_gradient_of_a_bias_and_of_a_weight_in_hbm():
     helpers.register_ramtorch_hook(v, lambda t: t * 2, helpers.ZERO2_HOOK_NAME)
     ck.linear(x, v).backward(gs[0])
     assert torch.equal(v.grad, dw_of(x, gs[0]) * 2)
+
+
+# ------------------------------------------------------------------------------------------- refusals
+@gpu
+def test_a_bias_of_another_type_or_shape_is_refused():
+    x, w = randn(T, K, seed=2), randn(N, K, seed=1)
+    for bias in (torch.zeros(N, device=DEV), torch.zeros(1, device=DEV, dtype=torch.bfloat16), torch.zeros(T, N, device=DEV, dtype=torch.bfloat16),
+                 torch.zeros(N + 1, device=DEV, dtype=torch.bfloat16), torch.zeros((), device=DEV, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="bias"):
+            ck.linear(x, w, bias)
