@@ -72,7 +72,7 @@ class _Linear(torch.autograd.Function):
                 gw = mx.weight_grad(grad, x8, dtype=weight.dtype)
                 gw = helpers.invoke_ramtorch_hooks(ctx.flagged[0], gw).to(weight.device)
         if ctx.bias_like is not None and ctx.needs_input_grad[2]:
-            gb = grad.reshape(-1, grad.shape[-1]).sum(0, dtype=torch.float32).to(ctx.bias_like["dtype"])
+            gb = grad.reshape(mx._split(grad.shape)).sum(0, dtype=torch.float32).to(ctx.bias_like["dtype"])
             gb = helpers.invoke_ramtorch_hooks(ctx.flagged[1], gb).to(ctx.bias_like["device"])
         return gx, gw, gb, None, None, None, None
 

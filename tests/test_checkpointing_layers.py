@@ -117,3 +117,13 @@ def test_a_bias_of_another_type_or_shape_is_refused():
                  torch.zeros(N + 1, device=DEV, dtype=torch.bfloat16), torch.zeros((), device=DEV, dtype=torch.bfloat16)):
         with pytest.raises(ValueError, match="bias"):
             ck.linear(x, w, bias)
+
+
+@gpu
+@pytest.mark.parametrize("product", [None, "mxfp4"])
+def test_a_layer_without_outputs(product):
+    x = randn(T, K, seed=2).requires_grad_()
+    w, b = torch.zeros(0, K, device=DEV, dtype=torch.bfloat16).requires_grad_(), torch.zeros(0, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    y = ck.linear(x, w, b, product=product)
+    y.backward(torch.zeros_like(y))
+    assert y.shape == (T, 0) and (x.grad == 0).all() and w.grad.shape == (0, K) and b.grad.shape == (0,)
