@@ -33,15 +33,16 @@ def _flagged(p: torch.Tensor | None):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
+    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, bias, product, seed, tensor_id, step):
         x = _rowed(x)
         w = weight if weight.is_cuda else weight.detach().to(x.device, non_blocking=True)
         if product == "mxfp4":
             y = mx.mxfp4_matmul(mx.quantize_mxfp4(x), mx.quantize_mxfp4(_rowed(w)), dtype=x.dtype)
         else:
-            y = x @ w.t()
+            y = x @ w.to(x.dtype).t()
         if bias is not None:
-            y = y + bias.to(x.device)
+            y = y + bias.to(x.device, x.dtype)
         keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] else None
         ctx.save_for_backward(*((keep.codes, keep.scales) if keep is not None else (None, None)), weight)
         # the parameters themselves: what is saved comes back as another tensor after recomputation or through saved-tensor hooks
@@ -51,6 +52,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @torch.amp.custom_bwd(device_type="cuda")
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         codes, scales, weight = ctx.saved_tensors
@@ -63,7 +65,7 @@ class _Linear(torch.autograd.Function):
                 d4 = mx.quantize_mxfp4(grad, seed=seed, tensor_id=tensor_id, step=step)
                 gx = mx.mxfp4_matmul(d4, mx.quantize_mxfp4(_rowed(w), transpose=True), dtype=ctx.x_dtype)
             else:
-                gx = grad @ w
+                gx = grad @ w.to(grad.dtype)
         if codes is not None:
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
             if ctx.flagged[0] is not None and not weight.is_cuda:
@@ -90,17 +92,24 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the
     flag, a cast or a slice of a parameter) goes to host memory through autograd.  ``AdamW.step`` takes
     ``rt_device_grad`` in place of ``grad``: a flagged parameter should get all of its gradient from one of the two.
-    ZeRO-2 hooks of flagged parameters see the fresh gradient, of a weight and of a bias, before it is added anywhere."""
+    ZeRO-2 hooks of flagged parameters see the fresh gradient, of a weight and of a bias, before it is added anywhere.
+
+    Under ``torch.autocast`` x is cast to its type, and y has that type; weight and bias may be of any of the three types,
+    and their gradients are formed in their own."""
     if product not in (None, "mxfp4"):
         raise ValueError(f"product must be None or 'mxfp4', not {product!r}")
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
-    if x.dtype != weight.dtype:
-        raise ValueError(f"x is {x.dtype} and weight {weight.dtype}")
-    if bias is not None and (bias.dtype != x.dtype or bias.shape != weight.shape[:1]):
-        raise ValueError(f"bias must be {x.dtype} of shape {tuple(weight.shape[:1])}, not {bias.dtype} {tuple(bias.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"bias must have shape {tuple(weight.shape[:1])}, not {tuple(bias.shape)}")
+    autocast = torch.is_autocast_enabled("cuda")
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None and (t.dtype not in mx.N.DTYPE_CODE if autocast else t.dtype != x.dtype):
+            raise ValueError(f"x is {x.dtype} and {name} {t.dtype}")
     if not x.is_cuda:
         raise RuntimeError("x must be a CUDA tensor: ramtorch_b200 has no CPU implementation")
+    if autocast and x.dtype in mx.N.DTYPE_CODE:
+        x = x.to(torch.get_autocast_dtype("cuda"))
     return _Linear.apply(x, weight, bias, product, seed, tensor_id, step)
 
 

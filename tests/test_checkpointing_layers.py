@@ -127,3 +127,66 @@ def test_a_layer_without_outputs(product):
     y = ck.linear(x, w, b, product=product)
     y.backward(torch.zeros_like(y))
     assert y.shape == (T, 0) and (x.grad == 0).all() and w.grad.shape == (0, K) and b.grad.shape == (0,)
+
+
+# --------------------------------------------------------------------------- automatic mixed precision
+@gpu
+@pytest.mark.parametrize("inside", [False, True])
+@pytest.mark.parametrize("product", [None, "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_under_autocast(dtype, product, inside):
+    """As torch's linear: inputs are cast, fp32 weights and biases get fp32 gradients.  Those come from the gradient of the cast
+    output and the checkpoint of the cast input, straight in fp32.  Two layers, the second on the first one's output."""
+    x = randn(T, K, seed=2, dtype=torch.float32).requires_grad_()
+    w1 = torch.nn.Parameter(randn(2 * N, K, seed=1, dtype=torch.float32) * 0.1)
+    w2 = torch.nn.Parameter(randn(K, N, seed=4, dtype=torch.float32) * 0.1)
+    b2 = torch.nn.Parameter(randn(K, seed=5, dtype=torch.float32))
+    gy = randn(T, K, seed=6, dtype=dtype)
+    with torch.autocast("cuda", dtype=dtype):
+        proj = ck.linear(x, w1, product=product)
+        h = ck.gated_act(*proj.chunk(2, -1))
+        y = ck.linear(h, w2, b2, product=product)
+        if inside:
+            grads = torch.autograd.grad(y, (x, w1, w2, b2, proj, h), gy)
+    assert proj.dtype == h.dtype == y.dtype == dtype
+    if not inside:
+        grads = torch.autograd.grad(y, (x, w1, w2, b2, proj, h), gy)
+    gx, g1, g2, gb, gproj, gh = grads
+    assert [t.dtype for t in grads] == [torch.float32] * 4 + [dtype] * 2
+    assert torch.equal(g2, dw_of(h, gy, torch.float32)) and torch.equal(g1, dw_of(x.to(dtype), gproj, torch.float32))
+    assert torch.equal(gb, gy.sum(0, dtype=torch.float32))
+    if product:
+        q = mx.quantize_mxfp4
+        assert torch.equal(proj, mx.mxfp4_matmul(q(x.to(dtype)), q(w1))) and torch.equal(gh, mx.mxfp4_matmul(q(gy), q(w2, transpose=True)))
+        assert torch.equal(gx, mx.mxfp4_matmul(q(gproj), q(w1, transpose=True)).float())
+    else:
+        assert torch.equal(proj, x.to(dtype) @ w1.to(dtype).t()) and torch.equal(gh, gy @ w2.to(dtype))
+        assert torch.equal(gx, (gproj @ w1.to(dtype)).float())
+
+
+@gpu
+def test_under_autocast_with_a_host_weight():
+    w, x, g = host_parameter(dtype=torch.float32), randn(T, K, seed=2, dtype=torch.float32), randn(T, N, seed=3)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = ck.linear(x, w)
+    assert torch.equal(y, x.bfloat16() @ w.detach().to(DEV).bfloat16().t())
+    y.backward(g)
+    assert torch.equal(held(w), dw_of(x.bfloat16(), g, torch.float32))
+
+
+@gpu
+def test_an_fp32_layer_whose_backward_pass_alone_is_under_autocast():
+    x, w, g = randn(T, K, seed=2, dtype=torch.float32).requires_grad_(), randn(N, K, seed=1, dtype=torch.float32).requires_grad_(), randn(T, N, seed=3, dtype=torch.float32)
+    y = ck.linear(x, w)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        gx, = torch.autograd.grad(y, (x,), g)
+    assert torch.equal(gx, g @ w)
+
+
+@gpu
+def test_types_that_differ_are_refused_without_autocast():
+    x, w = randn(T, K, seed=2), randn(N, K, seed=1, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        ck.linear(x, w)
+    with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(ValueError):
+        ck.linear(x, w.double())
