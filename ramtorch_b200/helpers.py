@@ -106,14 +106,15 @@ def accumulate_weight_grad(param: torch.Tensor, grad_out: torch.Tensor, x8) -> t
     ``grad_out.T @ x8`` from the layer's input as an MXINT8 checkpoint (``microscaling.quantize_mxint8``).
     The first micro-batch stores it in the parameter's dtype, later ones add in fp32 before the
     one rounding.  With ZeRO-2 hooks on the parameter the fresh gradient passes through them first
-    (linear.py:409-414), then is added.  Returns the accumulated gradient."""
+    (linear.py:409-414), then is added; so it is to what is held in another order of memory than by rows.  Returns the accumulated gradient."""
     from . import microscaling as mx
     if not grad_out.is_cuda:
         raise ValueError("accumulate_weight_grad is for gradients that live in HBM")
     if param.dim() != 2 or tuple(param.shape) != (grad_out.shape[-1], x8.shape[-1]):
         raise ValueError("gradient and parameter shapes differ")
     held = param.__dict__.get(DEVICE_GRAD_ATTR)
-    if held is not None and not getattr(param, ZERO2_HOOK_NAME, None):
+    rows = held is not None and held.stride(1) == 1 and held.stride(0) >= held.shape[1]      # what another producer left need not be
+    if rows and not getattr(param, ZERO2_HOOK_NAME, None):
         return mx.weight_grad(grad_out, x8, out=held, accumulate=True)
     fresh = mx.weight_grad(grad_out, x8, dtype=param.dtype)
     return accumulate_device_grad(param, invoke_ramtorch_hooks(param, fresh))

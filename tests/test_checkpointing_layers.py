@@ -87,6 +87,18 @@ def test_a_host_parameter_keeps_its_gradient_when_saved_tensors_are_packed(way):
     assert torch.equal(x.grad, plain)
 
 
+@gpu
+def test_a_held_gradient_in_any_order_of_memory_is_added_to():
+    """A gradient that another producer left on the parameter, its rows not runs of memory."""
+    w, x, g = host_parameter(), randn(T, K, seed=2), randn(T, N, seed=3)
+    first = randn(K, N, seed=4).t()
+    helpers.accumulate_device_grad(w, first.clone())
+    assert not held(w).is_contiguous()
+    want = first + dw_of(x, g)
+    ck.linear(x, w).backward(g)
+    assert torch.equal(held(w), want)
+
+
 # -------------------------------------------------------------------------------------- ZeRO-2 hooks
 @gpu
 def test_zero2_hooks_see_the_gradient_of_a_bias_and_of_a_weight_in_hbm():
