@@ -230,13 +230,18 @@ def _same_place(t, device, name):
         raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
+def _check_draws(tensor_id, step):
+    if not (0 <= tensor_id < 2**32 and 0 <= step < 2**32):
+        raise ValueError("tensor_id and step must fit 32 bits")
+
+
 def _quantize(x, fmt, transpose, seed, tensor_id, step):
     rows, cols, ld = _rows(x, "x")
     if transpose and x.dim() != 2:
         raise ValueError("transpose needs a matrix")
     shape = (cols, rows) if transpose else tuple(x.shape)
-    if seed is not None and not (0 <= tensor_id < 2**32 and 0 <= step < 2**32):
-        raise ValueError("tensor_id and step must fit 32 bits")
+    if seed is not None:
+        _check_draws(tensor_id, step)
     fast = _fast or _helper()
     if fast:
         codes, scales = fast.quantize(x, rows, cols, ld, _FORMATS[fmt], transpose, seed is not None, (seed or 0) & (2**64 - 1), tensor_id, step)

@@ -132,6 +132,14 @@ def test_a_bias_of_another_type_or_shape_is_refused():
 
 
 @gpu
+def test_draws_that_do_not_fit_are_refused_before_the_forward_pass():
+    x, w = randn(T, K, seed=2), randn(N, K, seed=1).requires_grad_()
+    for kw in (dict(step=-1), dict(step=2 ** 32), dict(tensor_id=-1), dict(tensor_id=2 ** 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ck.linear(x, w, product="mxfp4", seed=1, **kw)
+
+
+@gpu
 @pytest.mark.parametrize("product", [None, "mxfp4"])
 def test_a_layer_without_outputs(product):
     x = randn(T, K, seed=2).requires_grad_()
