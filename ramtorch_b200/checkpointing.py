@@ -98,7 +98,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     and their gradients are formed in their own."""
     if product not in (None, "mxfp4"):
         raise ValueError(f"product must be None or 'mxfp4', not {product!r}")
-    if seed is not None:
+    if product and seed is not None:
         mx._check_draws(tensor_id, step)
     if weight.dim() != 2 or x.dim() == 0 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
