@@ -879,9 +879,18 @@ static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, i
   auto encode = map_encoder();
   if (!encode) { cudaGetLastError(); return fail(RT_E_DEVICE, "the driver has no cuTensorMapEncodeTiled"); }
   const cuuint32_t ones[3] = {1, 1, 1};
-  const CUresult r = encode(map, type, (cuuint32_t)rank, const_cast<void*>(p), reinterpret_cast<const cuuint64_t*>(dims),
-                            reinterpret_cast<const cuuint64_t*>(strides), box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto fill = [&] {
+    return encode(map, type, (cuuint32_t)rank, const_cast<void*>(p), reinterpret_cast<const cuuint64_t*>(dims),
+                  reinterpret_cast<const cuuint64_t*>(strides), box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = fill();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {   // a thread's first call (autograd's, for one): the runtime has not bound the device's context yet
+    int device = 0;
+    RT_CUDA(cudaGetDevice(&device));
+    RT_CUDA(cudaSetDevice(device));
+    r = fill();
+  }
   if (r != CUDA_SUCCESS) return fail(RT_E_CONFIG, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
   return 0;
 }
