@@ -416,7 +416,7 @@ int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, con
 
 /* Waits inside the tensor-core kernels that ran out on the current device since load (each is bounded by
  * two seconds so that a fault ends the kernel instead of hanging the GPU).  0, or the results of a
- * call are wrong.  Synchronous. */
+ * call are wrong: what such a call did not form holds NaN.  Synchronous. */
 int rt_mx_wait_faults(uint32_t* count);
 
 /* out[m][n] = sum over k of the MXFP4 values a[m][k] * b[n][k]; fp32 sums, one rounding to out's type. */

@@ -47,6 +47,19 @@ __device__ __forceinline__ void put_out(const OutMatrix& o, int64_t at, float v)
   else if (o.dtype == RT_F32) put_one<RT_F32>(o, at, v);
   else put_one<RT_F16>(o, at, v);
 }
+// What is not formed because a wait ran out reads as NaN, so that no such result passes for one: column `col` of the
+// output in up to 32 rows from `row`, added to or not.
+template <typename T>
+__device__ __forceinline__ void fill_column(void* p, int64_t ld, int row, int rows, int col, T v) {
+  T* q = static_cast<T*>(p) + (int64_t)row * ld + col;
+#pragma unroll 1
+  for (int j = 0; j < 32 && row + j < rows; ++j) q[j * ld] = v;
+}
+__device__ __forceinline__ void put_nan(void* p, int64_t ld, int row, int rows, int col, int cols, int dtype) {
+  if (col >= cols) return;
+  if (dtype == RT_F32) fill_column<uint32_t>(p, ld, row, rows, col, 0x7FC00000u);
+  else fill_column<uint16_t>(p, ld, row, rows, col, dtype == RT_BF16 ? 0x7FC0 : 0x7E00);
+}
 // 16 columns of the accumulator that this warp holds, to 16 output rows
 template <int D>
 __device__ __forceinline__ void put_columns(const OutMatrix& o, int row, int col, const uint32_t (&acc)[16]) {
@@ -256,6 +269,14 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
           }
         }
       }
+    } else {
+#pragma unroll 1
+      for (int c = group * 32; c < BN; c += kGroups * 32) {
+        if (splits == 1) put_nan(o.p, o.ld, row0 + c, o.rows, col0 + q * 32 + lane, o.cols, o.dtype);
+        else
+#pragma unroll 1
+          for (int j = 0; j < 32; ++j) parts[(c + j) * 128 + q * 32 + lane] = __uint_as_float(0x7FC00000u);
+      }
     }
     tc_fence_before();
   }
@@ -419,7 +440,7 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
             mma_bf16<PAIR>(tmem + j * S::kN, da + kk * (2048 >> 4), db + ((j * kHalfN * kTok * 2 + kk * 2048) >> 4), idesc, i > 0 || kk > 0);
         tc_commit<PAIR>(empty + 8 * s, both);
       }
-      tc_commit<PAIR>(done, both);
+      if (ok) tc_commit<PAIR>(done, both);   // otherwise the workers' wait runs out too, and they leave NaN
     }
   } else if (warp == 3) {
     // the scales of a step: one word (four blocks) to a token
@@ -680,7 +701,7 @@ mx_fp4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__
                     sf + 8 + 4 * (kk >> 1), i > 0 || kk > 0);
         tc_commit<false>(empty + 8 * s);
       }
-      tc_commit<false>(done);
+      if (ok) tc_commit<false>(done);        // otherwise the workers' wait runs out too, and they leave NaN
     }
   } else if (warp >= kFirstWorker) {
     ok = mbar_wait_warp(done, 0);
@@ -803,7 +824,7 @@ mx_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_cons
           }
           tc_commit<true>(empty + 8 * s, 3);
         }
-        tc_commit<true>(done, 3);
+        if (ok) tc_commit<true>(done, 3);    // otherwise the workers' wait runs out too, and they leave NaN from this tile on
       }
     }
   } else if (warp >= kFirstWorker) {
@@ -814,9 +835,13 @@ mx_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_cons
     for (int t = blockIdx.x >> 1; t < tiles; t += pairs, ++n) {
       int m0, n0;
       place(t, m0, n0);
-      if (!(ok = mbar_wait_warp(done, n & 1))) break;
-      tc_fence_after();
       const int col = n0 + side * 128 + q * 32;
+      if (!(ok = ok && mbar_wait_warp(done, n & 1))) {
+#pragma unroll 1
+        for (int c = group * 32; c < S::kTileRows; c += 32 * kPairGroups) put_nan(a.out.p, a.out.ld, m0 + c, a.out.rows, col + lane, a.out.cols, a.out.dtype);
+        continue;
+      }
+      tc_fence_after();
 #pragma unroll 1
       for (int c = group * 32; c < S::kTileRows && m0 + c < a.out.rows; c += 32 * kPairGroups) {
         if (a.out.wide) {

@@ -280,6 +280,7 @@ def mxfp4_matmul(a: MxTensor, b: MxTensor, *, dtype=None, out: torch.Tensor | No
     if k != kb:
         raise ValueError(f"a has {k} columns and b {kb}")
     _same_place(b, a.device, "b")
+    _watched.setdefault(a.device.index, 0)
     shape = a.shape[:-1] + (n,)
     if out is None:
         dtype = _out_dtype(dtype or a.dtype)
@@ -296,6 +297,28 @@ def mxfp4_matmul(a: MxTensor, b: MxTensor, *, dtype=None, out: torch.Tensor | No
                                         out.data_ptr(), N.DTYPE_CODE[out.dtype], ld, N.stream_ptr(a.device.index)),
                 "rt_mxfp4_matmul")
     return out
+
+
+_watched: dict = {}        # devices that products ran on -> waits that had run out there when it was last asked
+
+
+def check_faults(device=None) -> None:
+    """Raise ``RuntimeError`` if a wait inside a product's kernel (:func:`mxfp4_matmul`, :func:`weight_grad`) has run out since
+    the last look, on `device` or on every device that had products.  Each wait is bounded by two seconds, so that a fault ends
+    the kernel instead of hanging the GPU; what such a call did not form holds NaN.  Waits for the device.
+    ``AdamW.step`` looks by itself where it waits anyway (``sync=True``)."""
+    if device is None:
+        asked = list(_watched)
+    else:
+        index = device if isinstance(device, int) else torch.device(device).index
+        asked = [torch.cuda.current_device() if index is None else index]
+    for index in asked:
+        count = ctypes.c_uint32()
+        with _on(torch.device("cuda", index)):
+            N.check(N.lib().rt_mx_wait_faults(ctypes.byref(count)), "rt_mx_wait_faults")
+        new, _watched[index] = count.value - _watched.get(index, 0), count.value
+        if new:
+            raise RuntimeError(f"{new} wait(s) inside the tensor-core kernels ran out on cuda:{index}: results of calls since the last look hold NaN")
 
 
 def _out_dtype(dtype):
@@ -325,6 +348,7 @@ def weight_grad(grad_out: torch.Tensor, x8: MxTensor, *, dtype=None, out: torch.
     if rows != tokens:
         raise ValueError(f"grad_out has {tokens} tokens and x8 {rows}")
     _same_place(x8, grad_out.device, "x8")
+    _watched.setdefault(grad_out.device.index, 0)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")

@@ -36,6 +36,7 @@ from torch.optim import Optimizer
 
 from .. import _native as N
 from .. import _shard_plan as SP
+from .. import microscaling as _mx
 from ..functional import sr_round_bf16_
 
 import contextlib
@@ -68,6 +69,13 @@ def _grad_of(p):
         if g is not None:
             return g
     return p.grad
+
+
+def _wait_for(index: int) -> None:
+    """Wait for the step on a device; where low-bit products ran there, their kernels are asked whether all went well."""
+    torch.cuda.current_stream(index).synchronize()
+    if index in _mx._watched:
+        _mx.check_faults(index)
 
 
 def copy_stochastic_(target: torch.Tensor, source: torch.Tensor, seed=0):
@@ -587,7 +595,7 @@ class AdamW(Optimizer):
         if self.sync:
             # results are visible to the host when step() returns (adamw.py:232)
             for index in used:
-                torch.cuda.current_stream(index).synchronize()
+                _wait_for(index)
             self._keepalive.clear()
         return loss
 
@@ -717,7 +725,7 @@ class AdamW(Optimizer):
             bucket.pushed = True
         self.last_step_info = dict(launches=plan.launches, resident=len(params), streamed=0, fast=True)
         if self.sync:
-            torch.cuda.current_stream(index).synchronize()
+            _wait_for(index)
         return True
 
     def _step_fast_scanned(self, lib, f, groups, all_params) -> bool:
@@ -766,7 +774,7 @@ class AdamW(Optimizer):
             bucket.pushed = True
         self.last_step_info = dict(launches=plan.launches, resident=len(states), streamed=0, fast=True)
         if self.sync:
-            torch.cuda.current_stream(index).synchronize()
+            _wait_for(index)
         return True
 
     def _row_means(self, lib, index, entries, rows_of, stream):
