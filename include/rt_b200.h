@@ -414,6 +414,16 @@ int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, con
                       int out_dtype, int64_t ld_out, int accumulate, void* workspace,
                       int64_t workspace_bytes, void* cuda_stream);
 
+/* How a product of these sizes runs on the current device: output rows to a tile, CTAs that share a tile (2: pairs),
+ * parts that a tile's sum is split into, and whether a second kernel joins those parts (otherwise a cluster
+ * does).  For tests and profiles; all 0 where nothing is launched. */
+typedef struct rt_mx_plan {
+  int32_t rows, ctas, splits, joined;
+} rt_mx_plan;
+int rt_mx_weight_grad_plan(const void* grad_out, int grad_dtype, int64_t ld_grad, int64_t tokens, int64_t n,
+                           int64_t k, rt_mx_plan* plan);
+int rt_mxfp4_matmul_plan(int64_t m, int64_t n, int64_t k, rt_mx_plan* plan);
+
 /* Waits inside the tensor-core kernels that ran out on the current device since load (each is bounded by
  * two seconds so that a fault ends the kernel instead of hanging the GPU).  0, or the results of a
  * call are wrong: what such a call did not form holds NaN.  Synchronous. */

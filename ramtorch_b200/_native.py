@@ -75,6 +75,10 @@ class MxDraws(ctypes.Structure):
     _fields_ = [("seed", c_uint64), ("tensor_id", c_uint32), ("step", c_uint32)]
 
 
+class MxPlan(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int32), ("ctas", ctypes.c_int32), ("splits", ctypes.c_int32), ("joined", ctypes.c_int32)]
+
+
 class Stats(ctypes.Structure):
     _fields_ = [("kernel_launches", c_uint64), ("h2d_bytes", c_uint64), ("d2h_bytes", c_uint64),
                 ("h2d_copies", c_uint64), ("d2h_copies", c_uint64)]
@@ -119,6 +123,8 @@ _SIGNATURES = {
     "rt_mx_weight_grad_workspace": (c_int64, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64]),
     "rt_mx_weight_grad": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
                                   c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "rt_mx_weight_grad_plan": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, ctypes.POINTER(MxPlan)]),
+    "rt_mxfp4_matmul_plan": (c_int, [c_int64, c_int64, c_int64, ctypes.POINTER(MxPlan)]),
     "rt_mx_wait_faults": (c_int, [ctypes.POINTER(c_uint32)]),
     "rt_mxfp4_matmul": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int,
                                 c_int64, c_void_p]),

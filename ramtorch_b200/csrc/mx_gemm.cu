@@ -1041,6 +1041,34 @@ static int fp4_pairs_at_once() {
   return clusters_at_once(mx_fp4_pair_kernel, known, kPairThreads, PairSmem::kBytes, 2);
 }
 
+// Tile and split of an MXFP4 product, by the microseconds that were measured for each: a start, then rounds of what runs
+// together.  Unsplit tiles run two to an SM and slow each other down; clusters run one CTA to an SM.
+// (4096 x 4096 x 4096: 45 us in 128 x 128 tiles, 38 in pairs; 2048 x 4096 x 4096: 23 and 25; 1 x 4096 x 4096:
+// 8.9 unsplit, 6.4 in four.)
+struct Fp4Plan {
+  int bm, splits;                         // bm: rows of a to a tile, 384 in pairs
+};
+static Fp4Plan plan_fp4(int64_t m, int64_t n, int steps) {
+  const int64_t n_tiles = (n + 127) / 128;
+  const int width = m <= 32 ? 32 : m <= 64 ? 64 : 128;      // narrow ones only for a single tile
+  const int64_t tiles = n_tiles * ((m + width - 1) / width);
+  Fp4Plan p{width, 1};
+  double best = 1e300;
+  for (int s = 1; s <= 8 && s <= steps; ++s) {
+    const int at_once = s == 1 ? 2 * kSms : width == 128 ? fp4_at_once<128>(s) : width == 64 ? fp4_at_once<64>(s) : fp4_at_once<32>(s);
+    const double both = s > 1 ? 0 : std::min(1.0, std::max(0.0, (double)(tiles - kSms) / kSms));     // how far tiles share an SM
+    const double round = (double)((steps + s - 1) / s) * (0.34 + 0.15 * both) + (s > 1 ? 3.0 : 1.2 + 1.5 * both);
+    const double cost = (s > 1 ? 2.0 : 2.5) + (double)((tiles + at_once - 1) / at_once) * round;
+    if (cost < best) { best = cost; p.splits = s; }
+  }
+  if (m > 128) {
+    const int64_t pair_tiles = (n + 255) / 256 * ((m + 383) / 384);
+    const int at_once = fp4_pairs_at_once();
+    if (3.5 + (double)((pair_tiles + at_once - 1) / at_once) * (steps * 0.5 + 3.0) < best) p = {384, 1};
+  }
+  return p;
+}
+
 static int pieces_of(int dtype) { return dtype == RT_F32 ? 3 : dtype == RT_F16 ? 2 : 1; }
 static bool taken_as_is(const void* p, int dtype, int64_t ld) { return dtype == RT_BF16 && aligned16(p, ld, 2); }
 
@@ -1056,6 +1084,29 @@ extern "C" int64_t rt_mx_weight_grad_workspace(const void* grad_out, int grad_dt
   const int pieces = taken_as_is(grad_out, grad_dtype, ld_grad) ? 0 : pieces_of(grad_dtype);
   const WgradPlan plan = plan_wgrad(tokens, n, k, std::max(1, pieces));
   return pad_to(pieces * tokens * pad_to(n, 8) * 2, 16) + (plan.joined ? plan.splits * n * pad_to(k, 4) * 4 : 0);
+}
+
+extern "C" int rt_mx_weight_grad_plan(const void* grad_out, int grad_dtype, int64_t ld_grad, int64_t tokens, int64_t n, int64_t k, rt_mx_plan* plan) {
+  if (!plan) return fail(RT_E_NULL, "plan must be non-null");
+  if (!dtype_ok(grad_dtype)) return fail(RT_E_DTYPE, "dtype code must be 0 (bf16), 1 (f32) or 2 (f16)");
+  if (int rc = mx_check_shape(tokens, k)) return rc;
+  if (int rc = mx_check_shape(tokens, n)) return rc;
+  *plan = rt_mx_plan{};
+  if (tokens == 0 || n == 0 || k == 0) return 0;
+  const WgradPlan p = plan_wgrad(tokens, n, k, taken_as_is(grad_out, grad_dtype, ld_grad) ? 1 : pieces_of(grad_dtype));
+  *plan = {p.bn, p.ctas, p.splits, p.joined};
+  return 0;
+}
+
+extern "C" int rt_mxfp4_matmul_plan(int64_t m, int64_t n, int64_t k, rt_mx_plan* plan) {
+  if (!plan) return fail(RT_E_NULL, "plan must be non-null");
+  if (int rc = mx_check_shape(m, k)) return rc;
+  if (int rc = mx_check_shape(n, k)) return rc;
+  *plan = rt_mx_plan{};
+  if (m == 0 || n == 0 || k == 0) return 0;
+  const Fp4Plan p = plan_fp4(m, n, (int)((pad_to(k, kMxBlock) + kStepK - 1) / kStepK));
+  *plan = {p.bm, p.bm == 384 ? 2 : 1, p.splits, 0};
+  return 0;
 }
 
 extern "C" int rt_mx_weight_grad(const void* grad_out, int grad_dtype, int64_t ld_grad, const void* codes, const void* scales,
@@ -1165,28 +1216,9 @@ extern "C" int rt_mxfp4_matmul(const void* a_codes, const void* a_scales, const 
   a.ktiles = (int)((kp + 127) / 128);
   a.out = {out, ld_out, (int)m, (int)n, out_dtype, 0, aligned16(out, ld_out, dtype_size(out_dtype))};
 
-  // Tile and split, by the microseconds that were measured for each: a start, then rounds of what runs
-  // together.  Unsplit tiles run two to an SM and slow each other down; clusters run one CTA to an SM.
-  // (4096 x 4096 x 4096: 45 us in 128 x 128 tiles, 38 in pairs; 2048 x 4096 x 4096: 23 and 25; 1 x 4096 x 4096:
-  // 8.9 unsplit, 6.4 in four.)
-  const int64_t n_tiles = (n + 127) / 128;
-  const int width = m <= 32 ? 32 : m <= 64 ? 64 : 128;      // rows of a to a tile: narrow ones only for a single tile
-  const int64_t tiles = n_tiles * ((m + width - 1) / width);
-  int bm = width, splits = 1;
-  double best = 1e300;
-  for (int s = 1; s <= 8 && s <= a.steps; ++s) {
-    const int at_once = s == 1 ? 2 * kSms : width == 128 ? fp4_at_once<128>(s) : width == 64 ? fp4_at_once<64>(s) : fp4_at_once<32>(s);
-    const double both = s > 1 ? 0 : std::min(1.0, std::max(0.0, (double)(tiles - kSms) / kSms));     // how far tiles share an SM
-    const double round = (double)((a.steps + s - 1) / s) * (0.34 + 0.15 * both) + (s > 1 ? 3.0 : 1.2 + 1.5 * both);
-    const double cost = (s > 1 ? 2.0 : 2.5) + (double)((tiles + at_once - 1) / at_once) * round;
-    if (cost < best) { best = cost; splits = s; }
-  }
-  const int64_t pair_tiles = (n + 255) / 256 * ((m + 383) / 384);
+  const int64_t n_tiles = (n + 127) / 128, pair_tiles = (n + 255) / 256 * ((m + 383) / 384);
   if (pair_tiles > 0x3FFFFFFFll) return fail(RT_E_SIZE, "m * n is too large");
-  if (m > 128) {
-    const int at_once = fp4_pairs_at_once();
-    if (3.5 + (double)((pair_tiles + at_once - 1) / at_once) * (a.steps * 0.5 + 3.0) < best) bm = 384;
-  }
+  const auto [bm, splits] = plan_fp4(m, n, a.steps);
   a.splits = splits;
   a.n_tiles = (int)n_tiles;
   a.m_tiles = (int)((m + bm - 1) / bm);

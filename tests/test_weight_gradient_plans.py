@@ -1,18 +1,21 @@
-"""The weight gradient from an 8-bit checkpoint, on whole numbers.
+"""The weight gradient from an 8-bit checkpoint, on whole numbers, in every tile shape and way of summing.
 
 Gradients and checkpoint values are small integers, so every partial sum is an integer below 2^24 and any order of
 additions gives the same bits: the result has to EQUAL the 64-bit one.  A step of the sum that is lost, taken twice, or
 meets the wrong tile of a ring shows at once, however long the sum."""
-import numpy as np
+import ctypes
+import math
+import random
+
 import pytest
 import torch
 
+from ramtorch_b200 import _native as N
 from ramtorch_b200 import microscaling as mx
 
 gpu = pytest.mark.gpu
 DEV = "cuda"
 TORCH = {"bf16": torch.bfloat16, "f32": torch.float32, "f16": torch.float16}
-PIECES = {"bf16": 1, "f16": 2, "f32": 3}      # bf16 numbers that add up to a value of the type
 
 
 def integers(rows, cols, top, seed, dtype=torch.float32):
@@ -44,3 +47,78 @@ def test_long_sums_of_whole_numbers_are_exact(tokens, n, k, kind):
         assert torch.equal(got.double(), exact)
     held = integers(n, k, 9, 5)
     assert torch.equal(mx.weight_grad(g, q, out=held.clone(), accumulate=True).double(), exact + held.double())
+
+
+# ---------------------------------------------------------------------------------------- every variant
+VARIANTS = [(512, "whole"), (512, "joined"), (256, "whole"), (256, "cluster"), (256, "joined"), (128, "whole"), (128, "cluster"), (128, "joined"),
+            (64, "whole"), (64, "cluster"), (64, "joined")]
+
+
+def plan_of(tokens, n, k, kind):
+    """(rows of a tile, how its sum is formed) of a gradient whose rows lie next to each other."""
+    p = N.MxPlan()
+    N.check(N.lib().rt_mx_weight_grad_plan(256, N.DTYPE_CODE[TORCH[kind]], n, tokens, n, k, ctypes.byref(p)))
+    assert p.ctas == (2 if p.rows >= 256 else 1)
+    return p.rows, "whole" if p.splits == 1 else "joined" if p.joined else "cluster"
+
+
+@pytest.fixture(scope="module")
+def shapes_of():
+    """Small shapes for every variant, found by asking: a rule that changes moves the shapes, and one that gives a variant up fails here."""
+    rng, found = random.Random(7), {v: [] for v in VARIANTS}
+    draw = lambda low, high: int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))      # noqa: E731
+    for _ in range(20000):
+        kind = rng.choice(["bf16", "bf16", "f32", "f16"])
+        t, n, k = draw(1, 20000), draw(1, 5000), draw(1, 9000)
+        if t * n * k < 2.5e9 and n * k < 2e7:
+            found[plan_of(t, n, k, kind)].append((t * n * k, t, n, k, kind))
+    return {v: sorted(s)[:: max(1, len(s) // 4)][:4] for v, s in found.items()}
+
+
+def view(rows, cols, kind, aligned):
+    """An output inside a buffer of sevens, its rows on 16-byte boundaries or not."""
+    buf = torch.full((rows + 2, (cols + 15) // 8 * 8 + (0 if aligned else 3)), 7.0, dtype=TORCH[kind], device=DEV)
+    return buf, buf[1:1 + rows, :cols] if aligned else buf[1:1 + rows, 1:1 + cols]
+
+
+def rest_is_sevens(buf, out):
+    out.fill_(7)
+    return bool((buf == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows,how", VARIANTS)
+def test_every_variant_is_exact(rows, how, shapes_of):
+    """Each tile shape and way of summing: all output types, on and off 16-byte boundaries, set and added."""
+    assert shapes_of[rows, how]
+    for _, tokens, n, k, kind in shapes_of[rows, how]:
+        assert plan_of(tokens, n, k, kind) == (rows, how)
+        g, q, exact = sums(tokens, n, k, kind, seed=tokens)
+        held = integers(n, k, 9, 5)
+        for out_kind in TORCH:
+            for aligned in (True, False):
+                for accumulate in (False, True):
+                    buf, out = view(n, k, out_kind, aligned)
+                    out.copy_(held)
+                    mx.weight_grad(g, q, out=out, accumulate=accumulate)
+                    want = (exact + held.double() if accumulate else exact).to(TORCH[out_kind])
+                    assert torch.equal(out, want), (tokens, n, k, kind, out_kind, aligned, accumulate)
+                    assert rest_is_sevens(buf, out)
+
+
+@gpu
+@pytest.mark.parametrize("tokens,n,k,kind,rows,how", [(2051, 1001, 4104, "bf16", 256, "whole"), (2048, 1024, 4096, "bf16", 256, "whole"), (8192, 4096, 11008, "bf16", 512, "whole"),
+                                                     (16384, 256, 512, "bf16", 128, "joined")])
+def test_plans_of_sizes_that_figures_are_given_for(tokens, n, k, kind, rows, how):
+    assert plan_of(tokens, n, k, kind) == (rows, how)
+
+
+def test_plan_queries_refuse():
+    p = N.MxPlan(1, 1, 1, 1)
+    lib = N.lib()
+    assert lib.rt_mx_weight_grad_plan(256, 0, 8, 2, 8, 8, None) == -1 and lib.rt_mxfp4_matmul_plan(2, 8, 8, None) == -1
+    assert lib.rt_mx_weight_grad_plan(256, 7, 8, 2, 8, 8, ctypes.byref(p)) == -2
+    assert lib.rt_mx_weight_grad_plan(256, 0, 8, -1, 8, 8, ctypes.byref(p)) == -3 and lib.rt_mxfp4_matmul_plan(2, -8, 8, ctypes.byref(p)) == -3
+    for call in (lambda: lib.rt_mx_weight_grad_plan(None, 0, 8, 0, 8, 8, ctypes.byref(p)), lambda: lib.rt_mxfp4_matmul_plan(2, 8, 0, ctypes.byref(p))):
+        p.rows = p.ctas = p.splits = p.joined = 1
+        assert call() == 0 and (p.rows, p.ctas, p.splits, p.joined) == (0, 0, 0, 0)      # nothing is launched
