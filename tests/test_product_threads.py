@@ -35,3 +35,33 @@ def test_products_are_the_first_call_of_a_thread(host_side, monkeypatch):
         want = call()               # plans and memory are there already
         torch.cuda.synchronize()
         assert torch.equal(in_a_new_thread(call), want)
+
+
+@pytest.mark.gpu
+def test_products_on_two_streams_and_in_two_threads_at_once():
+    """Every way of summing at the same time: nothing is shared between calls."""
+    r = lambda *s: torch.randn(*s, device="cuda").bfloat16()      # noqa: E731
+    g, q = r(4096, 130), mx.quantize_mxint8(r(4096, 200))           # parts that a second kernel joins
+    h, p = r(700, 1000), mx.quantize_mxint8(r(700, 600))
+    f = torch.randn(300, 200, device="cuda")
+    u = mx.quantize_mxint8(r(300, 100))                             # planes in a workspace
+    a, b, c = mx.quantize_mxfp4(r(3, 4096)), mx.quantize_mxfp4(r(900, 4096)), mx.quantize_mxfp4(r(1500, 4096))
+    calls = [lambda: mx.weight_grad(g, q), lambda: mx.weight_grad(h, p), lambda: mx.weight_grad(f, u), lambda: mx.mxfp4_matmul(a, b), lambda: mx.mxfp4_matmul(b, c)]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+
+    def run(order):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [(i, calls[i]()) for _ in range(20) for i in order]
+        stream.synchronize()
+        return all(torch.equal(t, want[i]) for i, t in got)
+
+    done = []
+    threads = [threading.Thread(target=lambda o=o: done.append(run(o))) for o in ((0, 1, 2, 3, 4), (4, 3, 2, 1, 0), (2, 4, 1, 3, 0))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert done == [True, True, True]
+    mx.check_faults()
