@@ -401,7 +401,7 @@ int rt_mx_gated_act_backward(const void* grad_h, int64_t ld_grad, int dtype, int
 /*
  * Weight gradient from a checkpoint: out[n][k] = sum over tokens t of grad_out[t][n] * value of the
  * MXINT8 matrix at [t][k] (what the reference's linear.py:401-412 computes from a saved 16-bit
- * input).  Every product is exact (an fp32 gradient enters down to 2^-133), sums are fp32, one rounding to out's type.  accumulate != 0 adds to
+ * input).  Every product is exact (an fp32 gradient enters down to 2^-133), sums are fp32 (the tensor core's, which cuts what does not fit), one rounding to out's type.  accumulate != 0 adds to
  * out instead (the sum in fp32, rounded once).  grad_out: tokens x n, row stride ld_grad; out: n x k,
  * row stride ld_out.  workspace: device memory of at least rt_mx_weight_grad_workspace(...) bytes
  * for the same arguments on the same device (often 0 for bf16 gradients whose rows start on 16-byte

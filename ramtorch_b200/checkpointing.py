@@ -86,7 +86,11 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``product=None``: the product and ``grad_x`` in x's own type.  ``product="mxfp4"``: both in 4-bit
     microscaled floating point; the incoming gradient is rounded to 4 bits stochastically when
     ``seed`` is given (Philox draws ``(seed, tensor_id, step)``: pass another ``tensor_id`` for each layer
-    and count ``step``), else to nearest.  The weight gradient always takes the gradient unrounded.
+    and count ``step`` with every call, micro-batches too; inside a CUDA graph each replay draws the same), else to
+    nearest.  The weight gradient always takes the gradient unrounded.
+
+    Every call keeps a copy of its own: projections of one input (q, k, v; gate, up) keep it once as one call with their
+    weights stacked, and once each as several.
 
     A weight in host memory is copied to x's device for the product.  The gradient of an ``is_ramtorch``
     parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the

@@ -262,7 +262,8 @@ struct SrArgs {
 
 // ------------------------------------------------------------------------------------- quantise
 // FMT 0: MXINT8, 1: MXFP4.  8192 x 11008 bf16: MXINT8 44 us (273 MB, 6.3 TB/s), MXFP4 41 us (228 MB, 5.5
-// TB/s, integer pipe 72 % busy).  Stochastic 88 us: the Philox rounds cost 29 of them and the rounding 18, on the same pipe.
+// TB/s, integer pipe 72 % busy).  Stochastic 86-88 us: the Philox rounds cost 29 of them and the rounding 18, on the same pipe; the
+// transposed kernel does the same in 77.  fp32: 69, 63 and 90 us; its aligned kernels spill up to 148 bytes at 40 registers.
 // Four rows to a thread (two: 50 us).
 constexpr int kRows = 4;   // rows to a thread
 
@@ -376,7 +377,7 @@ mx_quantize_t_kernel(const Matrix x, const int64_t rows, const int cols, const u
 }
 
 // ----------------------------------------------------------------------------------- the way back
-// 8192 x 11008 to bf16: MXINT8 45 us (273 MB, 6.1 TB/s), MXFP4 41 us.
+// 8192 x 11008 to bf16: MXINT8 45 us (273 MB, 6.1 TB/s), MXFP4 41 us; to fp16 48 and 47, to fp32 95 and 94.
 template <int D, int FMT, bool VEC>
 __global__ void __launch_bounds__(kMxThreads)
 mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Grid g, const Matrix out) {
@@ -472,7 +473,7 @@ struct Kept {              // an MXINT8 matrix
 
 // 8192 x 11008 bf16, silu: forward 110 us (727 MB, 6.6 TB/s), backward 109 us; gelu 130 and 132, gelu_tanh 120 forward.
 // Two rows to a thread: one or four lose 15 % to too few loads under way or too few warps.  Rows off 16-byte
-// boundaries (8191 x 11007): 136 and 171 us, gelu 169 and 196.
+// boundaries (8191 x 11007): 150 and 178 us, gelu 181 and 198.  fp32: 191 and 194 us, gelu 268 and 278.
 constexpr int kPairs = 2;  // rows to a thread
 
 template <int D, int ACT, bool VEC>

@@ -56,7 +56,7 @@ __device__ __forceinline__ float to_f32(elem_t<D> v) {
   else if constexpr (D == RT_BF16) return __uint_as_float((uint32_t)v << 16);
   else return __half2float(__ushort_as_half(v));
 }
-// round to nearest; finite values beyond fp16's range become its largest
+// round to nearest
 template <int D>
 __device__ __forceinline__ elem_t<D> of_f32(float v) {
   if constexpr (D == RT_F32) return v;

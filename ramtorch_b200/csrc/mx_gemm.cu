@@ -21,7 +21,7 @@ int mx_check_codes(const void* codes, const void* scales);
 
 __device__ unsigned int g_wait_faults;   // waits that ran out; see rt_mx_wait_faults
 
-constexpr int kSms = 148;
+constexpr int kSms = 148;                 // of a B200; how many clusters run at once is asked of the device
 constexpr int kFirstWorker = 4;          // warp 0: loads, 1: products, 2: tensor memory, 3: scales, from 4: conversion and output
 constexpr int kConvGroups = 2;           // of four warps each, in the weight gradient's kernel
 constexpr int kWgradThreads = 32 * (kFirstWorker + 4 * kConvGroups);
@@ -321,9 +321,12 @@ __device__ __forceinline__ void finish_tile(const OutMatrix& o, uint32_t tmem, i
 // products; both CTAs' workers arrive at its barrier.
 //
 // What bounds it: at BN = 512 (all of tensor memory; a step's converted tile serves two products) the
-// tensor core, 472-481 us at 8192 x 4096 x 11008 = 1540-1560 TFLOP/s (taking out the conversion changed nothing); below that
+// tensor core, 472-482 us at 8192 x 4096 x 11008 = 1530-1560 TFLOP/s (taking out the conversion changed nothing); below that
 // the conversion, some 0.4 us a step (8192 codes; four integer operations to a pair, and the pipe
-// takes a warp in two clocks): 18 us at 2048 x 1024 x 4096, 14 at 16384 x 256 x 512.
+// takes a warp in two clocks): 18.8 us at 2048 x 1024 x 4096, 14.8 at 16384 x 256 x 512.
+// The sums are what the tensor core makes of them: it cuts the bits that do not fit, so that an fp32 result comes out
+// a little small.  Off by (relative norm, normal data, 4096 x 4096 outputs) 2e-7 at 1024 tokens, 2.7e-6 at 8192, 7e-6 at 16384, as
+// the library's bf16 product with fp32 results is to the digit; where the sum is split, as the shorter sums are.
 constexpr int kTok = 64;
 
 template <int BN, bool PAIR>
@@ -528,7 +531,8 @@ mx_weight_grad_kernel(const __grid_constant__ CUtensorMap map_codes, const __gri
 
 // Few tiles and a long sum: more splits than a cluster has CTAs, each leaving its part of the output in
 // fp32, and this kernel adds them up in their order.  Four columns to a thread.  65536 x 256 x 512: 25 us
-// (in clusters of eight, which run 15 at a time, 54), 16384 x 256 x 512: 14 (18).
+// (in clusters of eight, which run 15 at a time, 54), 16384 x 256 x 512: 14.8 (18).  18 parts of 256 x 512 take it 3 us, bound by
+// the latency of its loads.
 __global__ void __launch_bounds__(256)
 join_parts_kernel(const float4* __restrict__ parts, const int64_t quads, const int splits, const FastDiv per_row, const OutMatrix o) {
   const uint32_t q = blockIdx.x * 256 + threadIdx.x;
@@ -550,6 +554,8 @@ join_parts_kernel(const float4* __restrict__ parts, const int64_t quads, const i
 // A gradient that the tensor maps cannot take as it is (fp32, fp16, rows that do not start on 16-byte
 // boundaries) as bf16 planes whose sum it is (down to 2^-133, the last place of a bf16 number): the
 // leading 8 bits of each value's mantissa, the next 8, the rest.  Cut, not rounded, so that nothing overflows; an infinity or a NaN is in the first plane alone.
+// 4096 x 4096 fp32: 24 us, bound by the integer pipe (66 %) and memory (67 MB read, 100 written); the planes cost more in what follows, the
+// codes being widened once for each: 4096 x 4096 x 1024 takes 103-115 us from fp32, 78-82 from fp16.
 // Eight values of a row to a thread, of two rows, planes of np = n rounded up to eight columns.
 template <int D, int P, bool VEC>
 __global__ void __launch_bounds__(256)
@@ -605,7 +611,7 @@ static void run_spread(const void* g, int64_t ld, int64_t tokens, int64_t n, voi
 // two copies (one per 128 columns) to tensor memory, where each stage has columns of its own.
 // The product takes a tile's scales from where a scale tile begins (an odd column of tensor memory
 // is a misaligned address to it), so narrow tiles serve only matrices of a single tile of rows.
-// One token against 11008 x 4096: 9 us (24 MB at 2.7 TB/s).  What bounds it there is the chain of a step, 0.34 us:
+// One token against 11008 x 4096: 8.2-8.6 us (24 MB at 2.8-2.9 TB/s).  What bounds it there is the chain of a step, 0.34 us:
 // scales, four products that add to the same sums, release; twice the loads under way changed nothing.
 constexpr int kStepK = 256;
 
@@ -1016,7 +1022,7 @@ static WgradPlan plan_wgrad(int64_t tokens, int64_t n, int64_t k, int pieces) {
     }
     const int64_t s = std::min<int64_t>(c.at_once(c.ctas) / tiles, steps / 2);
     if (s >= 2 && s * n * k <= ((int64_t)1 << 26)) {
-      const double cost = (double)((steps + s - 1) / s) * c.step + c.fixed + 3500 + (double)(s * n * k) * 8 / 8000;     // written and read in L2
+      const double cost = (double)((steps + s - 1) / s) * c.step + c.fixed + 3500 + (double)(s * n * k) * 8 / 8000;     // written and read; fitted to parts that stay in L2
       if (cost < best) { best = cost; p = {c.bn, c.ctas, (int)s, true, k_tiles, n_tiles}; }
     }
   }

@@ -1,7 +1,8 @@
 // Host side of the microscaled calls in C++: allocates the results, makes the inputs' device current,
 // and calls the C ABI on the current stream.  Shapes, strides and types have been checked by
 // ramtorch_b200/microscaling.py, which does the same through ctypes when this module is not built;
-// what this saves is Python time (12 us a call down to 7), which is most of a small call.
+// what this saves is Python time (quantize_mxint8 13.0 us a call down to 9.8, weight_grad 16.8 to 10.1, gated_act 36 to 16), which
+// is most of a small call.
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
