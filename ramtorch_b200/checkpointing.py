@@ -31,6 +31,18 @@ def _flagged(p: torch.Tensor | None):
     return p if p is not None and p.is_leaf and getattr(p, "is_ramtorch", False) else None
 
 
+def _asked(ctx, i: int):
+    """Whether this backward pass wants the gradient of tensor input `i`: ``"added"`` to the parameter, ``"returned"``
+    (``torch.autograd.grad`` for the parameter itself), or None (``autograd.grad`` or ``backward(inputs=...)`` for others)."""
+    node = ctx.next_functions[i][0]
+    if node is None:
+        return None
+    try:
+        return "added" if torch._C._will_engine_execute_node(node) else None
+    except RuntimeError:                # a leaf whose gradient autograd.grad captures
+        return "returned"
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
@@ -66,16 +78,20 @@ class _Linear(torch.autograd.Function):
                 gx = mx.mxfp4_matmul(d4, mx.quantize_mxfp4(_rowed(w), transpose=True), dtype=ctx.x_dtype)
             else:
                 gx = grad @ w.to(grad.dtype)
-        if codes is not None:
+        if codes is not None and (asked := _asked(ctx, 1)):
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
-            if ctx.flagged[0] is not None and not weight.is_cuda:
+            if asked == "added" and ctx.flagged[0] is not None and not weight.is_cuda:
                 helpers.accumulate_weight_grad(ctx.flagged[0], grad, x8)
             else:
                 gw = mx.weight_grad(grad, x8, dtype=weight.dtype)
-                gw = helpers.invoke_ramtorch_hooks(ctx.flagged[0], gw).to(weight.device)
-        if ctx.bias_like is not None and ctx.needs_input_grad[2]:
+                if asked == "added":
+                    gw = helpers.invoke_ramtorch_hooks(ctx.flagged[0], gw)
+                gw = gw.to(weight.device)
+        if ctx.bias_like is not None and ctx.needs_input_grad[2] and (asked := _asked(ctx, 2)):
             gb = grad.reshape(mx._split(grad.shape)).sum(0, dtype=torch.float32).to(ctx.bias_like["dtype"])
-            gb = helpers.invoke_ramtorch_hooks(ctx.flagged[1], gb).to(ctx.bias_like["device"])
+            if asked == "added":
+                gb = helpers.invoke_ramtorch_hooks(ctx.flagged[1], gb)
+            gb = gb.to(ctx.bias_like["device"])
         return gx, gw, gb, None, None, None, None
 
 

@@ -210,3 +210,21 @@ def test_types_that_differ_are_refused_without_autocast():
         ck.linear(x, w)
     with torch.autocast("cuda", dtype=torch.bfloat16), pytest.raises(ValueError):
         ck.linear(x, w.double())
+
+
+@gpu
+def test_a_gradient_that_is_not_asked_for_is_not_added():
+    """``torch.autograd.grad`` and ``backward(inputs=...)`` add to nothing else, host parameters included."""
+    w, b, x, g = host_parameter(), torch.nn.Parameter(randn(N, seed=9, device="cpu")), randn(T, K, seed=2).requires_grad_(), randn(T, N, seed=3)
+    b.is_ramtorch, seen = True, []
+    helpers.register_ramtorch_hook(b, lambda t: seen.append(t), helpers.ZERO2_HOOK_NAME)
+    layer = lambda: ck.linear(x, w, b)      # noqa: E731
+    torch.autograd.grad(layer(), (x,), g)
+    layer().backward(g, inputs=[x])
+    assert held(w) is None and w.grad is None and b.grad is None and not seen
+    got, = torch.autograd.grad(layer(), (w,), g)
+    assert torch.equal(got, dw_of(x, g).cpu()) and held(w) is None and w.grad is None and not seen
+    layer().backward(g, inputs=[w])
+    assert torch.equal(held(w), dw_of(x, g)) and w.grad is None and b.grad is None
+    layer().backward(g)
+    assert len(seen) == 1 and torch.equal(b.grad, g.sum(0, dtype=torch.float32).bfloat16().cpu())
