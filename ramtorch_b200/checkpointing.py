@@ -43,6 +43,19 @@ def _asked(ctx, i: int):
         return "returned"
 
 
+def _ready_for_caller(held: torch.Tensor) -> None:
+    """What autograd does for ``.grad``: when this backward pass is over, the stream it was called on is ordered after the stream
+    that `held` was written on (the forward pass's)."""
+    stream = torch.cuda.current_stream(held.device)
+
+    def order():
+        caller = torch.cuda.current_stream(held.device)
+        if caller != stream:
+            caller.wait_stream(stream)
+            held.record_stream(caller)
+    torch.autograd.Variable._execution_engine.queue_callback(order)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     @torch.amp.custom_fwd(device_type="cuda")
@@ -81,7 +94,7 @@ class _Linear(torch.autograd.Function):
         if codes is not None and (asked := _asked(ctx, 1)):
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
             if asked == "added" and ctx.flagged[0] is not None and not weight.is_cuda:
-                helpers.accumulate_weight_grad(ctx.flagged[0], grad, x8)
+                _ready_for_caller(helpers.accumulate_weight_grad(ctx.flagged[0], grad, x8))
             else:
                 gw = mx.weight_grad(grad, x8, dtype=weight.dtype)
                 if asked == "added":

@@ -228,3 +228,27 @@ def test_a_gradient_that_is_not_asked_for_is_not_added():
     assert torch.equal(held(w), dw_of(x, g)) and w.grad is None and b.grad is None
     layer().backward(g)
     assert len(seen) == 1 and torch.equal(b.grad, g.sum(0, dtype=torch.float32).bfloat16().cpu())
+
+
+@gpu
+@pytest.mark.parametrize("reentrant", [None, True])
+def test_a_held_gradient_is_ready_where_backward_was_called(reentrant):
+    """As of ``.grad``: a forward pass on another stream, whose work is late, and a reader on the stream that called backward."""
+    w, x, g = host_parameter(), randn(T, K, seed=2), randn(T, N, seed=3)
+    want = dw_of(x, g)
+    ck.linear(x, w).backward(g)                       # what is there before is another gradient
+    side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+    for add in (False, True):
+        if not add:
+            w.rt_device_grad = None
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            y = ck.linear(x, w)
+            if reentrant:
+                a = x.detach().requires_grad_()
+                y = checkpoint(lambda a: ck.linear(a, w), a, use_reentrant=True)
+            torch.cuda._sleep(200_000_000)            # a tenth of a second before the backward pass can run there
+        y.backward(g)
+        got = held(w).clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, mx.weight_grad(g, mx.quantize_mxint8(x), out=want.clone(), accumulate=True) if add else want)
