@@ -25,6 +25,14 @@ def _rowed(t: torch.Tensor) -> torch.Tensor:
         return t.contiguous()
 
 
+def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """``a @ b`` in their own type, also where autocast is on when the backward pass is called."""
+    if torch.is_autocast_enabled("cuda"):
+        with torch.autocast("cuda", enabled=False):
+            return a @ b
+    return a @ b
+
+
 def _flagged(p: torch.Tensor | None):
     """`p` if it is an ``is_ramtorch`` parameter itself, else None.  What was made of a parameter (a cast, a slice) has to
     pass its gradient on through autograd."""
@@ -46,26 +54,26 @@ def _asked(ctx, i: int):
 def _ready_for_caller(held: torch.Tensor) -> None:
     """What autograd does for ``.grad``: when this backward pass is over, the stream it was called on is ordered after the stream
     that `held` was written on (the forward pass's)."""
-    stream = torch.cuda.current_stream(held.device)
+    index = held.get_device()
+    written_on = mx.N.stream_ptr(index)
 
     def order():
-        caller = torch.cuda.current_stream(held.device)
-        if caller != stream:
-            caller.wait_stream(stream)
+        if mx.N.stream_ptr(index) != written_on:
+            caller = torch.cuda.current_stream(index)
+            caller.wait_stream(torch.cuda.ExternalStream(written_on, index))
             held.record_stream(caller)
     torch.autograd.Variable._execution_engine.queue_callback(order)
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    @torch.amp.custom_fwd(device_type="cuda")
     def forward(ctx, x, weight, bias, product, seed, tensor_id, step):
         x = _rowed(x)
         w = weight if weight.is_cuda else weight.detach().to(x.device, non_blocking=True)
         if product == "mxfp4":
             y = mx.mxfp4_matmul(mx.quantize_mxfp4(x), mx.quantize_mxfp4(_rowed(w)), dtype=x.dtype)
         else:
-            y = x @ w.to(x.dtype).t()
+            y = _product(x, w.to(x.dtype).t())
         if bias is not None:
             y = y + bias.to(x.device, x.dtype)
         keep = mx.quantize_mxint8(x) if ctx.needs_input_grad[1] else None
@@ -77,7 +85,6 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.amp.custom_bwd(device_type="cuda")
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         codes, scales, weight = ctx.saved_tensors
@@ -90,7 +97,7 @@ class _Linear(torch.autograd.Function):
                 d4 = mx.quantize_mxfp4(grad, seed=seed, tensor_id=tensor_id, step=step)
                 gx = mx.mxfp4_matmul(d4, mx.quantize_mxfp4(_rowed(w), transpose=True), dtype=ctx.x_dtype)
             else:
-                gx = grad @ w.to(grad.dtype)
+                gx = _product(grad, w.to(grad.dtype))
         if codes is not None and (asked := _asked(ctx, 1)):
             x8 = mx.MxTensor("mxint8", codes, scales, ctx.x_shape, ctx.x_dtype)
             if asked == "added" and ctx.flagged[0] is not None and not weight.is_cuda:
@@ -124,7 +131,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     A weight in host memory is copied to x's device for the product.  The gradient of an ``is_ramtorch``
     parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the
     flag, a cast or a slice of a parameter) goes to host memory through autograd.  ``AdamW.step`` takes
-    ``rt_device_grad`` in place of ``grad``: a flagged parameter should get all of its gradient from one of the two.
+    ``rt_device_grad`` in place of ``grad`` and ``AdamW.zero_grad`` clears it: a flagged parameter should get all of its gradient
+    from one of the two, and ``Module.zero_grad``, ``clip_grad_norm_`` and ``GradScaler``, which know ``grad`` alone, want it unflagged.
     ZeRO-2 hooks of flagged parameters see the fresh gradient, of a weight and of a bias, before it is added anywhere.
 
     Under ``torch.autocast`` x is cast to its type, and y has that type; weight and bias may be of any of the three types,
