@@ -128,7 +128,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     Every call keeps a copy of its own: projections of one input (q, k, v; gate, up) keep it once as one call with their
     weights stacked, and once each as several.
 
-    A weight in host memory is copied to x's device for the product.  The gradient of an ``is_ramtorch``
+    A weight in host memory is copied to x's device for the product, asynchronously where it is pinned.  The gradient of an ``is_ramtorch``
     parameter stays there as ``weight.rt_device_grad``; that of any other host weight (a leaf without the
     flag, a cast or a slice of a parameter) goes to host memory through autograd.  ``AdamW.step`` takes
     ``rt_device_grad`` in place of ``grad`` and ``AdamW.zero_grad`` clears it: a flagged parameter should get all of its gradient
